@@ -121,7 +121,8 @@ def _tokens(g, shape, dtype, outliers):
 def _code(x, codes):
     """x [..., 64, D] -> (codes as float32, scales [...]): the operator's definition, in 32 bits."""
     x = x.float()
-    scale = (x.abs().amax((-2, -1)) / TOP[codes]).clamp_min(2.0 ** -126)
+    amax = x.abs().amax((-2, -1))
+    scale = (amax / torch.full_like(amax, TOP[codes])).clamp_min(2.0 ** -126)  # (a Python divisor would be a multiplication)
     y = x * (1.0 / scale)[..., None, None]
     y = y.clamp(-TOP[codes], TOP[codes])
     return (y.to(torch.float8_e4m3fn) if codes == "e4m3" else torch.round(y).to(torch.int8)), scale
