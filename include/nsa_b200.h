@@ -271,6 +271,85 @@ int nsa_kivi_stream_decode_step_layers(const nsa_kivi_stream_cache* caches, int6
                                        void* const* o, float sm_scale, void* workspace, size_t workspace_bytes,
                                        nsa_stream_t stream);
 
+/* ------------------------------------------------------------------ 8-bit
+ * Paged KV cache held in 8 bits, with a scale for each block of 64 tokens and
+ * head (no reference counterpart: the reference quantizes a window to 2 bits,
+ * quant_kernel.py:584-622).  One attention layer; D is 64 or 128; any number
+ * of query heads per KV head; float16 or bfloat16 tokens, queries and outputs.
+ *
+ *   codes   u8 [n_pages, Hkv, 64, D], K and V apart: a page holds one block,
+ *           64 consecutive tokens, of every head; float8 e4m3 or int8 values
+ *   scales  f32 [n_pages, Hkv, 2]: the block's K and V scale
+ *   table   int32 [batch, max_blocks]: page of a sequence's block
+ *   ring    f16/bf16 [batch, Hkv, 128, D], K and V apart: position p at slot
+ *           p % 128 holds the tokens of the incomplete block as they came, and
+ *           keeps those of the block before it
+ *   lens    int64 [batch]: tokens of each sequence
+ *
+ * Complete blocks are read as codes, the up to 63 tokens behind them from the
+ * ring, so what the cache holds depends on the tokens alone, not on how calls
+ * cut them.  scale = max(amax / top, 2^-126) with top = 448 (e4m3) or 127
+ * (int8); code = x * (1 / scale) in float32, rounded to nearest even; value =
+ * scale * code.  A value that is not finite is kept as NaN; its block's scale
+ * is then NaN, and attention that sees it is NaN.
+ *
+ * Pages may be shared by sequences (equal table entries) as long as no call
+ * completes a shared block.  A page number outside [0, n_pages), a length or
+ * start outside the table's room, and a start that the ring no longer reaches
+ * are recorded in the device error word as NSA_ERR_INVALID: an append then
+ * leaves that sequence (for a page number: that block) as it was, attention
+ * over a bad page is NaN, over a bad length 0. */
+enum { NSA_KV8_E4M3 = 0, NSA_KV8_INT8 = 1 };
+typedef struct {
+  int64_t batch, n_kv_heads, head_dim, n_pages, max_blocks;
+  int32_t dtype;       /* of ring, new tokens, q and o: 1 = float16, 2 = bfloat16 */
+  int32_t codes;       /* NSA_KV8_E4M3 or NSA_KV8_INT8 */
+  void *k_codes, *v_codes;
+  float* scales;
+  int32_t* page_table;
+  void *k_ring, *v_ring;
+  int64_t* lens;
+  int64_t* ring_floor; /* int64 [batch], zero-filled once: oldest position the ring still holds */
+  int32_t* tickets;    /* int32 [batch], zero-filled once; left zero */
+} nsa_kv8_cache;
+/* Rows of head_dim elements; strides in elements (multiples of 8, data
+ * 16-byte aligned, so that every row is too). */
+typedef struct {
+  void* data;
+  int64_t batch_stride, head_stride, token_stride;
+} nsa_kv8_rows;
+
+/* Write counts[b] (NULL: all n_tokens) tokens of new_k / new_v [batch, Hkv,
+ * n_tokens, D] at positions starts[b] (NULL: lens[b]) on, quantize the blocks
+ * that this completes and set lens[b] = start + count.  A start below lens
+ * takes tokens back: any multiple of 64, or a position in the block in which
+ * the last append of tokens ended or the one before it. */
+int nsa_kv8_append(const nsa_kv8_cache* cache, const nsa_kv8_rows* new_k, const nsa_kv8_rows* new_v, int64_t n_tokens,
+                   const int64_t* starts, const int64_t* counts, nsa_stream_t stream);
+/* Read positions starts[b] (NULL: 0) .. + n_tokens of every sequence back into
+ * contiguous k_out / v_out [batch, Hkv, n_tokens, D] of out_dtype (0 =
+ * float32, 1 = float16, 2 = bfloat16); positions outside [0, lens[b]) are 0. */
+int nsa_kv8_read(const nsa_kv8_cache* cache, int64_t n_tokens, const int64_t* starts, void* k_out, void* v_out,
+                 int out_dtype, nsa_stream_t stream);
+/* Attention of the last counts[b] (NULL: all n_tokens, at most 64) tokens of
+ * every sequence: row i of q [batch, n_heads, n_tokens, D] stands at position
+ * lens[b] - counts[b] + i and sees the positions p up to its own, with window
+ * >= 0 only those with p < sink or p > own - window (window < 0: all).  Rows
+ * that see nothing, and rows i >= counts[b], are 0.  Deterministic.
+ * workspace: nsa_kv8_workspace_bytes bytes of any contents, 16-byte aligned.
+ * tickets: nsa_kv8_ticket_count() int32, zero-filled once; left zero.  Neither
+ * may be shared by calls that can run concurrently. */
+size_t nsa_kv8_workspace_bytes(const nsa_kv8_cache* cache, int64_t n_heads, int64_t n_tokens);
+int64_t nsa_kv8_ticket_count(void);
+int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_kv8_rows* o, int64_t n_heads,
+                   int64_t n_tokens, const int64_t* counts, int64_t window, int64_t sink, float sm_scale,
+                   void* workspace, size_t workspace_bytes, int32_t* tickets, nsa_stream_t stream);
+/* nsa_kv8_append of the n_tokens, then nsa_kv8_attend of their queries. */
+int nsa_kv8_decode_step(const nsa_kv8_cache* cache, const nsa_kv8_rows* new_k, const nsa_kv8_rows* new_v,
+                        const nsa_kv8_rows* q, const nsa_kv8_rows* o, int64_t n_heads, int64_t n_tokens,
+                        const int64_t* starts, const int64_t* counts, int64_t window, int64_t sink, float sm_scale,
+                        void* workspace, size_t workspace_bytes, int32_t* tickets, nsa_stream_t stream);
+
 /* ------------------------------------------------------------ host buffers
  * Decode entry points over HOST buffers, for callers whose queries and
  * outputs live in host memory (the reference's Python functions accept CPU

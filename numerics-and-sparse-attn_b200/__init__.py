@@ -12,6 +12,7 @@ from .decode import (RingCache, dense_decode_attention, dense_decode_attention_h
                      sparse_decode_attention_host)
 from .kivi import (KiviCache, build_quantized_kv_cache, decode_step_layers, dequantize_k, dequantize_v,
                    quantize_k_cache, quantize_v_cache, sparse_decode_attention_quantized)
+from .kv8 import Kv8Cache
 
 __all__ = [
     "dense_decode_attention",
@@ -25,6 +26,7 @@ __all__ = [
     "KiviCache",
     "decode_step_layers",
     "RingCache",
+    "Kv8Cache",
     "HostPipe",
     "dense_decode_attention_host",
     "sparse_decode_attention_host",

@@ -60,6 +60,12 @@ PROTOTYPES = {
     "nsa_ring_append": (_INT, [_P, _P, _P, _P, _P] + [_I64] * 5 + [_P]),
     "nsa_ring_decode": (_INT, [_P, _P, _P, _P] + [_I64] * 6 + [_P, _F, _P, _SZ, _P]),
     "nsa_ring_decode_step": (_INT, [_P, _P, _P, _P] + [_I64] * 6 + [_P, _P, _P, _F, _P, _SZ, _P]),
+    "nsa_kv8_append": (_INT, [_P, _P, _P, _I64, _P, _P, _P]),
+    "nsa_kv8_read": (_INT, [_P, _I64, _P, _P, _P, _INT, _P]),
+    "nsa_kv8_workspace_bytes": (_SZ, [_P, _I64, _I64]),
+    "nsa_kv8_ticket_count": (_I64, []),
+    "nsa_kv8_attend": (_INT, [_P, _P, _P, _I64, _I64, _P, _I64, _I64, _F, _P, _SZ, _P, _P]),
+    "nsa_kv8_decode_step": (_INT, [_P] * 5 + [_I64, _I64, _P, _P, _I64, _I64, _F, _P, _SZ, _P, _P]),
     "nsa_host_pipe_create": (_P, [_SZ, _SZ, _INT]),
     "nsa_host_pipe_destroy": (None, [_P]),
     "nsa_host_pipe_begin": (_INT, [_P, _P]),

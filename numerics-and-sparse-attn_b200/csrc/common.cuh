@@ -106,6 +106,13 @@ __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.p
 // ---------------------------------------------------------------- TMA
 // Tiled tensor loads into this CTA's shared memory, completion counted in
 // bytes on an mbarrier.  Plain (non-multicast) form only.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
                                             int c0, int c1, int c2) {
   asm volatile(

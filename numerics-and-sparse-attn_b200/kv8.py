@@ -1,0 +1,253 @@
+"""Host side of the 8-bit paged KV cache.
+
+``Kv8Cache`` holds one attention layer's whole context in 8 bits (float8 e4m3
+or int8), with a scale for each block of 64 tokens and head, in pages that a
+table assigns to the sequences: half the bytes of a 16-bit cache for decode to
+read.  The up to 63 tokens behind a sequence's last complete block stay in
+16 bits, so what the cache holds depends on the tokens alone.  The layout and
+semantics are documented with ``nsa_kv8_cache`` in include/nsa_b200.h; the
+reference has no counterpart.
+
+Beside the other caches: ``KiviCache`` keeps a window at 2 bits, ``RingCache``
+a window at 16 bits, ``Kv8Cache`` every token (and attends to all of them or
+to sink + window).  It takes float16 or bfloat16, head_dim 64 or 128, any
+number of query heads per KV head, ragged batches and several query tokens.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .constants import D_HEAD, SINK_SIZE
+
+BLOCK = 64    # tokens of a page and of a scale
+RING = 128    # 16-bit slots of a sequence: the incomplete block and the one before it
+MAX_QUERY = 64  # query tokens of one attend
+
+_CODES = {"e4m3": (0, torch.float8_e4m3fn), "int8": (1, torch.int8)}
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_GRAPH_SLOTS = 256
+
+
+def _req(cond, msg, exc=ValueError):
+    if not cond:
+        raise exc(msg)
+
+
+class Kv8CacheDesc(ctypes.Structure):
+    """ctypes mirror of nsa_kv8_cache (include/nsa_b200.h)."""
+    _fields_ = [(n, ctypes.c_int64) for n in ("batch", "n_kv_heads", "head_dim", "n_pages", "max_blocks")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "codes")] + \
+               [(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "scales", "page_table", "k_ring", "v_ring", "lens",
+                                               "ring_floor", "tickets")]
+
+
+class Kv8Rows(ctypes.Structure):
+    """ctypes mirror of nsa_kv8_rows."""
+    _fields_ = [("data", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("batch_stride", "head_stride",
+                                                                           "token_stride")]
+
+
+def _rows(t):
+    """[B, H, D] or [B, H, T, D] as nsa_kv8_rows; dimensions of one element have no stride."""
+    shape, st = t.shape, t.stride()
+    return ctypes.byref(Kv8Rows(t.data_ptr(), st[0] if shape[0] > 1 else 0, st[1] if shape[1] > 1 else 0,
+                                st[2] if len(shape) == 4 and shape[2] > 1 else 0))
+
+
+class Kv8Cache:
+    """8-bit paged KV cache of one attention layer.
+
+    ``batch`` sequences of up to ``max_len`` tokens.  ``n_pages`` None: every
+    sequence has pages of its own; else a pool of that many pages, which the
+    caller hands out by writing page numbers into ``page_table`` (int32
+    [batch, blocks], initially 0) before a block is completed.  Sequences may
+    share pages of complete blocks.  ``lens`` (int64 [batch]) holds the lengths.
+
+    Storage, readable at any time: ``k_codes`` / ``v_codes`` [n_pages, Hkv, 64,
+    D] (float8_e4m3fn or int8), ``scales`` [n_pages, Hkv, 2] float32 (K, V),
+    ``k_ring`` / ``v_ring`` [batch, Hkv, 128, D] (position p at slot p % 128).
+
+    Calls on one cache are ordered by their stream; calls that write (append,
+    decode_step, truncate) must not overlap other calls on the cache.  A page
+    number outside the pool, a length or start outside the table's room and a
+    start that the ring no longer reaches are reported by ``device_error()``.
+    """
+
+    def __init__(self, batch, n_kv_heads, max_len, head_dim=D_HEAD, dtype=torch.float16, codes="e4m3", n_pages=None,
+                 device=None):
+        _req(head_dim in (64, 128), f"head_dim must be 64 or 128, got {head_dim}")
+        _req(dtype in (torch.float16, torch.bfloat16), f"dtype must be float16 or bfloat16, got {dtype}", TypeError)
+        _req(codes in _CODES, f"codes must be 'e4m3' or 'int8', got {codes!r}")
+        batch, n_kv_heads, max_len = int(batch), int(n_kv_heads), int(max_len)
+        _req(batch >= 0 and n_kv_heads > 0 and max_len > 0, "need batch >= 0, n_kv_heads > 0 and max_len > 0")
+        _req(n_pages is None or n_pages >= 1, "n_pages must be positive")
+        device = torch.device(device if device is not None else "cuda")
+        _req(device.type == "cuda", "Kv8Cache lives on a CUDA device (no CPU fallback)")
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.batch, self.n_kv_heads, self.head_dim, self.dtype, self.codes = batch, n_kv_heads, head_dim, dtype, codes
+        self.max_blocks = (max_len + BLOCK - 1) // BLOCK
+        self.n_pages = max(1, batch * self.max_blocks) if n_pages is None else int(n_pages)
+        self.device = device
+        code, form = _CODES[codes]
+
+        def z(shape, dt):
+            return torch.zeros(shape, dtype=dt, device=device)
+
+        page = (self.n_pages, n_kv_heads, BLOCK, head_dim)
+        ring = (batch, n_kv_heads, RING, head_dim)
+        self.k_codes, self.v_codes, self.scales = z(page, form), z(page, form), z(page[:2] + (2,), torch.float32)
+        self.k_ring, self.v_ring = z(ring, dtype), z(ring, dtype)
+        self.page_table = z((batch, self.max_blocks), torch.int32)
+        if n_pages is None:
+            self.page_table.copy_(torch.arange(batch * self.max_blocks, dtype=torch.int32).view(batch, -1))
+        self.lens, self._ring_floor = z((batch,), torch.int64), z((batch,), torch.int64)
+        self._append_tickets = z((batch,), torch.int32)
+        d = self._desc = Kv8CacheDesc(batch, n_kv_heads, head_dim, self.n_pages, self.max_blocks, _DTYPES[dtype], code)
+        for n, t in (("k_codes", self.k_codes), ("v_codes", self.v_codes), ("scales", self.scales),
+                     ("page_table", self.page_table), ("k_ring", self.k_ring), ("v_ring", self.v_ring),
+                     ("lens", self.lens), ("ring_floor", self._ring_floor), ("tickets", self._append_tickets)):
+            setattr(d, n, t.data_ptr())
+        self._desc_ref = ctypes.byref(d)
+        lib = _lib.load()
+        with _lib.on_device(device):
+            self._n_tickets = int(lib.nsa_kv8_ticket_count())
+        self._graph_tickets = z((_GRAPH_SLOTS, self._n_tickets), torch.int32)
+        self._graph_calls = 0
+        self._ws_bytes, self._eager = {}, {}
+
+    # ---------------------------------------------------------------- plumbing
+    def _check(self, name, t, heads):
+        """Checks [B, heads, D] or [B, heads, T, D]; returns T."""
+        _req(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor", TypeError)
+        _req(t.device == self.device, f"{name} must be a CUDA tensor on the cache's device {self.device} (no CPU fallback)")
+        _req(t.dtype == self.dtype, f"{name} must be {self.dtype}, got {t.dtype}", TypeError)
+        shape = t.shape
+        _req(len(shape) in (3, 4) and shape[0] == self.batch and shape[-1] == self.head_dim
+             and (shape[1] == heads if heads else shape[1] > 0 and shape[1] % self.n_kv_heads == 0),
+             f"{name} must be [{self.batch}, {heads or f'multiple of {self.n_kv_heads}'}, (T,) {self.head_dim}], "
+             f"got {tuple(shape)}")
+        _req(t.stride(-1) == 1, f"the last dimension of {name} must be contiguous")
+        return shape[2] if len(shape) == 4 else 1
+
+    def _words(self, name, t):
+        """Device pointer of an optional int64 [B] tensor."""
+        if t is None:
+            return None
+        _req(isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.device == self.device
+             and t.shape == (self.batch,) and t.is_contiguous(),
+             f"{name} must be a contiguous int64 CUDA tensor of length B on the cache's device")
+        return t.data_ptr()
+
+    def _scratch(self, heads, n_tokens, stream):
+        """Workspace and tickets of one attend.  Eager calls: one pair per
+        stream.  A call captured into a graph: workspace from the graph's own
+        pool and a ticket row of its own (256 rows, then from the start again),
+        so that graphs replayed side by side do not share them."""
+        key = (heads, n_tokens)
+        nbytes = self._ws_bytes.get(key)
+        if nbytes is None:
+            nbytes = _lib.load().nsa_kv8_workspace_bytes(self._desc_ref, heads, n_tokens)
+            if self.batch and not nbytes:
+                _lib.check(_lib.NSA_ERR_INVALID)  # raises with the library's message
+            self._ws_bytes[key] = nbytes
+        if torch.cuda.is_current_stream_capturing():
+            tickets = self._graph_tickets[self._graph_calls % _GRAPH_SLOTS]
+            self._graph_calls += 1
+            return torch.empty(nbytes, dtype=torch.uint8, device=self.device), tickets
+        pair = self._eager.get(stream)
+        if pair is None or pair[0].numel() < nbytes:
+            tickets = pair[1] if pair else torch.zeros(self._n_tickets, dtype=torch.int32, device=self.device)
+            pair = self._eager[stream] = (torch.empty(nbytes, dtype=torch.uint8, device=self.device), tickets)
+        return pair
+
+    def _mask(self, window, sink):
+        window, sink = -1 if window is None else int(window), int(sink)
+        _req(window >= -1 and sink >= 0, "window and sink must not be negative")
+        return window, sink
+
+    # ---------------------------------------------------------------- writing
+    def append(self, new_k, new_v, counts=None, starts=None):
+        """Write new tokens behind each sequence's, quantizing every block that
+        they complete.  new_k / new_v: [B, Hkv, D] or [B, Hkv, T, D] (any strides
+        with the last dimension contiguous).  ``counts`` (int64 [B]): of the T
+        tokens, how many each sequence takes; ``starts`` (int64 [B]): positions
+        to write at instead of ``lens``, so that a start below it takes tokens
+        back (any multiple of 64, or as far as the block before the one in
+        which the last append ended)."""
+        t = self._check("new_k", new_k, self.n_kv_heads)
+        _req(self._check("new_v", new_v, self.n_kv_heads) == t and new_v.dim() == new_k.dim(),
+             "new_k and new_v must have the same shape")
+        with _lib.on_device(self.device):
+            _lib.check(_lib.load().nsa_kv8_append(self._desc_ref, _rows(new_k), _rows(new_v), t,
+                                                  self._words("starts", starts), self._words("counts", counts),
+                                                  _lib.stream_handle(self.device)))
+
+    def truncate(self, lens):
+        """Set the lengths to ``lens`` (int64 [B]), taking tokens back as
+        ``append``'s ``starts`` does (0 empties a sequence)."""
+        with _lib.on_device(self.device):
+            _lib.check(_lib.load().nsa_kv8_append(self._desc_ref, None, None, 0, self._words("lens", lens), None,
+                                                  _lib.stream_handle(self.device)))
+
+    # ---------------------------------------------------------------- reading
+    def read(self, n_tokens, starts=None, dtype=None):
+        """The tokens at positions starts[b] (default 0) .. + n_tokens as attention
+        sees them: (k, v) [B, Hkv, n_tokens, D] of ``dtype`` (float32, float16
+        or bfloat16; default the cache's).  Positions outside a sequence are 0."""
+        dtype = self.dtype if dtype is None else dtype
+        _req(dtype in _DTYPES, f"dtype must be float32, float16 or bfloat16, got {dtype}", TypeError)
+        n_tokens = int(n_tokens)
+        _req(n_tokens >= 0, "n_tokens must not be negative")
+        k, v = (torch.empty((self.batch, self.n_kv_heads, n_tokens, self.head_dim), dtype=dtype, device=self.device)
+                for _ in range(2))
+        with _lib.on_device(self.device):
+            _lib.check(_lib.load().nsa_kv8_read(self._desc_ref, n_tokens, self._words("starts", starts), k.data_ptr(),
+                                                v.data_ptr(), _DTYPES[dtype], _lib.stream_handle(self.device)))
+        return k, v
+
+    # ---------------------------------------------------------------- attention
+    def attend(self, q, sm_scale=None, window=None, sink=SINK_SIZE, counts=None):
+        """Attention of the sequences' last tokens -> o like q.
+
+        q: [B, H, D], each sequence's last token, or [B, H, T, D] (T <= 64), its
+        last T: row i stands at position lens - T + i and sees the tokens up to
+        its own; with ``window`` only the newest ``window`` of them and the
+        first ``sink``.  ``counts`` (int64 [B]): how many of the T query tokens
+        each sequence has (row i then at lens - counts + i).  Rows that see
+        nothing and rows behind counts are 0."""
+        t = self._check("q", q, 0)
+        heads = q.shape[1]
+        window, sink = self._mask(window, sink)
+        o = torch.empty_like(q)
+        with _lib.on_device(self.device):
+            stream = _lib.stream_handle(self.device)
+            ws, tickets = self._scratch(heads, t, stream)
+            _lib.check(_lib.load().nsa_kv8_attend(
+                self._desc_ref, _rows(q), _rows(o), heads, t, self._words("counts", counts), window, sink,
+                self.head_dim ** -0.5 if sm_scale is None else float(sm_scale), ws.data_ptr(), ws.numel(),
+                tickets.data_ptr(), stream))
+        return o
+
+    def decode_step(self, q, new_k, new_v, sm_scale=None, window=None, sink=SINK_SIZE, counts=None, starts=None):
+        """append(new_k, new_v, counts, starts), then attend(q, ...) with the
+        new tokens as queries: q [B, H, D] with new_k / new_v [B, Hkv, D], or
+        all three with T tokens."""
+        t = self._check("q", q, 0)
+        _req(self._check("new_k", new_k, self.n_kv_heads) == t and self._check("new_v", new_v, self.n_kv_heads) == t,
+             "q, new_k and new_v must hold the same number of tokens")
+        heads = q.shape[1]
+        window, sink = self._mask(window, sink)
+        o = torch.empty_like(q)
+        with _lib.on_device(self.device):
+            stream = _lib.stream_handle(self.device)
+            ws, tickets = self._scratch(heads, t, stream)
+            _lib.check(_lib.load().nsa_kv8_decode_step(
+                self._desc_ref, _rows(new_k), _rows(new_v), _rows(q), _rows(o), heads, t,
+                self._words("starts", starts), self._words("counts", counts), window, sink,
+                self.head_dim ** -0.5 if sm_scale is None else float(sm_scale), ws.data_ptr(), ws.numel(),
+                tickets.data_ptr(), stream))
+        return o
