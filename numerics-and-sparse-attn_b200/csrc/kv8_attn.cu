@@ -15,17 +15,16 @@
 // of 64 or 128 rows; here the conversion happens in registers on the way from
 // ldmatrix to the mma.
 //
-// Work is split evenly over persistent CTAs (two per SM) by items: an item is
-// a block of 64 tokens, or a sequence's incomplete block (from the ring).  The
-// lengths live on the device, so every CTA computes the split itself (one scan
-// over the batch).  A CTA's consecutive items form pieces of units (sequence,
-// KV head, 32-row tile); a unit cut between CTAs is merged by the last of them to
-// finish.  In a CTA one warp feeds a ring of TMA stages and four consume:
-// a warp scores 16 of an item's 64 tokens for all rows, the four agree on the rows'
-// maxima and exchange P through shared memory, and each accumulates a quarter
-// of the head dimension over all 64 tokens.  So the accumulators of a piece
-// need no merge between warps (short sequences end often), and they stay at
-// 8 registers per 8 rows.
+// Work is split evenly over independent workers by steps: a step is 32 or 64
+// tokens of a block (8 KiB of codes), or 16 or 32 tokens of a sequence's
+// incomplete block in the ring.  The lengths live on the device, so every CTA
+// computes the split itself (one scan over the batch).  A worker is one warp
+// (up to 16 query rows) or 2 or 4 warps (32, 64 rows) that share its copies; it
+// issues its own TMA loads, two or more steps ahead, and keeps scores, P and
+// accumulators in registers, so no warp waits for another until its steps are
+// done.  A worker's consecutive steps form pieces of units (sequence, KV head,
+// row tile).  Units cut between workers are merged by the CTA at its end, and
+// those cut between CTAs by the last of them to finish.
 #include <cstddef>
 #include <cstdlib>
 
@@ -35,36 +34,51 @@ namespace nsa {
 namespace kv8 {
 namespace {
 
-constexpr int kWarps = 4;  // consumers
-constexpr int kThreads = (kWarps + 1) * 32;
-constexpr int kCtasPerSm = 2;
-constexpr int kRowTile = 32;   // query rows of a unit at most
-constexpr int kLensCached = 512;  // sequence lengths kept in shared memory
+constexpr uint32_t kHalf = 4096;     // bytes of K, and of V, in a stage
+constexpr uint32_t kStageBytes = 2 * kHalf;
+constexpr int kLensCached = 1024;    // sequence lengths kept in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendParams {
   Cache c;
   Rows q, o;
   int group, n_tokens, rows, row_tiles;  // rows = n_tokens * group of a KV head
+  uint32_t group_inv;                    // ceil(2^32 / group)
   const int64_t* counts;
   int window, sink;  // window < 0: all positions
   float scale_log2;
-  int n_ctas;
-  int* tickets;    // [n_ctas]
-  float* partials;  // [n_ctas][2] pieces of 8 * NT rows: m, l, then kD sums a row
+  int* tickets;     // [CTAs]
+  float* partials;  // [workers][2] pieces, then [CTAs][2]: m and l of every row, then kD sums a row
   int* err;
+};
+
+// n / group; exact for n < 2^16, group <= 2^10 (the error of group_inv adds
+// less than n / 2^32 to a quotient that is at least 1 / group below the next).
+__device__ __forceinline__ int token_of(const AttendParams& p, int n) {
+  return p.group == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), p.group_inv));
+}
+
+template <int kD>
+struct Geo {
+  static constexpr int kTok = kHalf / kD;          // tokens of a block step
+  static constexpr int kSteps = kBlock / kTok;     // steps of a block
+  static constexpr int kRingTok = kHalf / (2 * kD);  // tokens of a ring step
+  static constexpr uint32_t kRegions = kD / 64;    // 128-byte column parts of a ring step
+  static constexpr uint32_t kRegion = kRingTok * 128;
 };
 
 // One sequence as the kernel sees it.
 struct Seq {
-  int len, cnt;       // tokens; query tokens (rows of later ones are 0)
-  int full;           // complete blocks
-  int sink_blocks, win_block;  // block items: [0, sink_blocks), [win_block, full)
-  int items;          // at least 1
-  bool empty;         // nothing to see: its one item writes zeros
+  int len, cnt;                // tokens; query tokens (rows of later ones are 0)
+  int full;                    // complete blocks
+  int sink_blocks, win_block;  // blocks read: [0, sink_blocks), [win_block, full)
+  int steps;                   // at least 1
+  bool empty;                  // nothing to see: its one step writes zeros
 };
 
+template <int kD>
 __device__ __forceinline__ Seq make_seq(const AttendParams& p, int len, int cnt) {
+  using G = Geo<kD>;
   Seq s;
   s.len = len;
   s.cnt = cnt;
@@ -75,14 +89,14 @@ __device__ __forceinline__ Seq make_seq(const AttendParams& p, int len, int cnt)
     s.sink_blocks = min((p.sink + kBlock - 1) / kBlock, s.full);
     s.win_block = min(max(max(len - cnt + 1 - p.window, 0) / kBlock, s.sink_blocks), s.full);
   }
-  s.items = s.sink_blocks + s.full - s.win_block + (len % kBlock != 0);
-  s.empty = cnt == 0 || s.items == 0;
-  if (s.empty) s.items = 1;
+  s.steps = (s.sink_blocks + s.full - s.win_block) * G::kSteps + (len % kBlock + G::kRingTok - 1) / G::kRingTok;
+  s.empty = cnt == 0 || s.steps == 0;
+  if (s.empty) s.steps = 1;
   return s;
 }
 
-// A sequence's length and query count as one word (both checked): an invalid
-// length reads as an empty sequence.
+// A sequence's length and query count, checked: an invalid one reads as an
+// empty sequence.
 __device__ __forceinline__ int2 load_len(const AttendParams& p, int b) {
   const int64_t len = p.c.lens[b];
   const int64_t cnt = p.counts ? p.counts[b] : p.n_tokens;
@@ -93,36 +107,57 @@ __device__ __forceinline__ int2 load_len(const AttendParams& p, int b) {
   return make_int2(static_cast<int>(len), static_cast<int>(cnt));
 }
 
-template <int kD>
-struct Geo {
-  static constexpr uint32_t kCodeBytes = kBlock * kD;         // K (or V) codes of a block
-  static constexpr uint32_t kStageBytes = 2 * kCodeBytes;     // also 32 ring tokens of K and V
-  static constexpr uint32_t kRegions = kD / 64;               // 128-byte column halves of a ring tile
-  static constexpr uint32_t kRegion = 32 * 128;               // 32 ring rows of one half
-  static constexpr int kQStride = kD * 2 + 32;                // bytes: rows 8 banks apart
+// What a worker has to know of a staged step.
+struct alignas(16) Step {
+  int b, sub;    // sequence; KV head * row_tiles + row tile
+  int pos0;      // position of its first token
+  int flags;     // kFirst..., and from bit 8 on the tokens of a ring step
+  int len, cnt;  // of the sequence
+  int step, steps;  // of its unit
+  float ks, vs;  // scales
+  int pad[2];
+};
+enum : int {
+  kFirst = 1,   // of the worker's piece
+  kLast = 2,
+  kBegin = 4,   // of the unit
+  kEnd = 8,
+  kRingStep = 16,
+  kEmpty = 32,
+  kMasked = 64  // some row does not see some of its tokens
 };
 
-constexpr int kPStride = kBlock * 2 + 16;  // bytes of a row of P: rows 4 banks apart
+// A worker's part of a cut unit.
+struct Part {
+  int unit_begin;  // the unit's first step
+  float* data;
+  int b, sub, cnt, steps;
+  int flags;  // 0: none; else kFirst and whether it holds the unit's begin / end
+};
 
-template <int kD, int kNT>
+// Warps of a CTA (one per SM), warps of a worker, stages of a worker: 24 stages
+// of 8 KiB in flight an SM.
+template <int kNT, int kR>
+struct Shape {
+  static constexpr int kWarps = kNT == 1 ? 12 : 8;
+  static constexpr int kWorkers = kWarps / kR;
+  static constexpr int kStages = 24 / kWorkers;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kRows = 8 * kNT * kR;  // of a unit
+};
+
+template <int kNT, int kR>
 struct Smem {
-  static constexpr int kStages = (kNT == 1 ? 6 : 5) * (128 / kD);  // 80-96 KiB in flight a CTA
-  uint8_t stage[kStages][Geo<kD>::kStageBytes];  // 1024-aligned: TMA destinations
-  uint8_t q[2][8 * kNT][Geo<kD>::kQStride];
-  uint8_t p_hi[8 * kNT][kPStride];
-  uint8_t p_lo[8 * kNT][kPStride];
-  float q_scale[8 * kNT];
-  float mx[kWarps][8 * kNT];  // rows' maxima over each warp's tokens; sums at a piece's end
-  float2 scale[kStages];
+  using H = Shape<kNT, kR>;
+  uint8_t stage[H::kWorkers][H::kStages][kStageBytes];  // 1024-aligned: TMA destinations
+  Step step[H::kWorkers][H::kStages];
+  Part part[H::kWorkers][2];
   int2 lens[kLensCached];
-  int scan[kThreads / 32];
-  int b0, base_hi, base_lo;  // first sequence of this CTA, items before it
-  int ticket;
-  uint64_t full[kStages], empty[kStages];
-  uint64_t q_full[2], q_empty[2];
+  int scan[H::kWarps];
+  int before[H::kThreads];  // steps before a thread's sequences
+  int last[2];  // whether this CTA was the last of its first / last cut unit
+  uint64_t full[H::kWorkers][H::kStages], empty[H::kWorkers][H::kStages];
 };
-
-__device__ __forceinline__ void sync_consumers() { asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory"); }
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -173,23 +208,6 @@ __device__ __forceinline__ uint32_t lds4(uint32_t addr) {
   return x;
 }
 
-// Stores x as a 16-bit number at byte `at` of p_hi and, with `split`, what
-// that rounding left at `at` of p_lo.
-template <bool kBf16, class SmemT>
-__device__ __forceinline__ void store_p(SmemT& sm, uint32_t at, float x, bool split) {
-  uint8_t* hi = &sm.p_hi[0][0] + at;
-  uint8_t* lo = &sm.p_lo[0][0] + at;
-  if constexpr (kBf16) {
-    const __nv_bfloat16 y = __float2bfloat16_rn(x);
-    *reinterpret_cast<__nv_bfloat16*>(hi) = y;
-    if (split) *reinterpret_cast<__nv_bfloat16*>(lo) = __float2bfloat16_rn(x - __bfloat162float(y));
-  } else {
-    const __half y = __float2half_rn(x);
-    *reinterpret_cast<__half*>(hi) = y;
-    if (split) *reinterpret_cast<__half*>(lo) = __float2half_rn(x - __half2float(y));
-  }
-}
-
 // A pair of fp16 numbers of 8 significant bits as bf16 (exact).  volatile, so
 // that the conversions of all query fragments stay on the ring's path instead
 // of being kept in registers.
@@ -208,169 +226,92 @@ __device__ __forceinline__ bool sees(const AttendParams& p, int pos, int lim) {
   return pos < lim && (p.window < 0 || pos < p.sink || pos >= lim - p.window);
 }
 
-// The values of an incomplete block (ring slots in stages st and st1, 32
-// each; `tail` of them hold tokens, pos0 is the first's position) times P, for
-// the warp's head dimensions: blk = V^T P^T.  Rows of P are split in two.
-template <int kD, int kNT, bool kBf16, class SmemT, class LimitOf>
-__device__ __forceinline__ void ring_values(const SmemT& sm, const AttendParams& p, uint32_t st, uint32_t st1, int tail,
-                                            int pos0, int warp, int lane, LimitOf limit_of, int n0, uint32_t ph,
-                                            uint32_t pl, float (&blk)[kNT][kD / 64][4]) {
-  using G = Geo<kD>;
-  constexpr int kMT = kD / 64;
-  const int g = lane >> 2, t = lane & 3;
-  for (int kk = 0; kk < 2 && 32 * kk < tail; ++kk) {
-    const uint32_t vb = smem_u32(sm.stage[kk ? st1 : st]) + G::kCodeBytes;
-    uint32_t a[2][kMT][4];
-    uint32_t bad = 0;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int c = 0; c < kMT; ++c) {
-        const int cc = kMT * warp + c;  // 16-wide chunk of the head dimension
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9: dims 2g, 2g + 1
-          const uint32_t row = 16 * i + 2 * t + (e & 1) + (e >> 1) * 8;
-          w[e] = lds4(vb + (cc >> 2) * G::kRegion + row * 128 + ((((cc & 3) * 2 + (g >> 2)) ^ (row & 7)) << 4) +
-                      (g & 3) * 4);
-          if (32 * kk + static_cast<int>(row) >= tail) w[e] = 0u;  // no token: whatever the slot held
-          bad |= nonfinite_mask<kBf16>(w[e]);
-        }
-        a[i][c][0] = __byte_perm(w[0], w[1], 0x5410);
-        a[i][c][1] = __byte_perm(w[0], w[1], 0x7632);
-        a[i][c][2] = __byte_perm(w[2], w[3], 0x5410);
-        a[i][c][3] = __byte_perm(w[2], w[3], 0x7632);
-      }
-    const bool any_bad = __any_sync(0xffffffffu, bad != 0);
-    if (any_bad) {
-      // Values that are not finite would reach rows that do not see them (0 *
-      // NaN).  They are taken out, and a product of their places with the
-      // rows' masks says which sums they make NaN.
-      const uint32_t one = kBf16 ? 0x3f803f80u : 0x3c003c00u;
-      uint32_t ind[2][kMT][4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int c = 0; c < kMT; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t mk = nonfinite_mask<kBf16>(a[i][c][e]);
-            ind[i][c][e] = one & mk;
-            a[i][c][e] &= ~mk;
-          }
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        const int lim = limit_of(n0 + 8 * nt + g);
-        float hit[kMT][4];
-#pragma unroll
-        for (int c = 0; c < kMT; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) hit[c][e] = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t b[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int pos = pos0 + 32 * kk + 16 * i + 2 * t + 8 * e;
-            b[e] = one & ((sees(p, pos, lim) ? 0xffffu : 0u) | (sees(p, pos + 1, lim) ? 0xffff0000u : 0u));
-          }
-#pragma unroll
-          for (int c = 0; c < kMT; ++c)
-            mma_elem<kBf16>(hit[c], ind[i][c][0], ind[i][c][1], ind[i][c][2], ind[i][c][3], b[0], b[1]);
-        }
-#pragma unroll
-        for (int c = 0; c < kMT; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (hit[c][e] > 0.f) blk[nt][c][e] = NAN;
-      }
-    }
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      uint32_t b[4], b2[4];
-      ldmatrix_x4(ph + nt * 8 * kPStride + kk * 64, b[0], b[1], b[2], b[3]);
-      ldmatrix_x4(pl + nt * 8 * kPStride + kk * 64, b2[0], b2[1], b2[2], b2[3]);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int c = 0; c < kMT; ++c) {
-          mma_elem<kBf16>(blk[nt][c], a[i][c][0], a[i][c][1], a[i][c][2], a[i][c][3], b[2 * i], b[2 * i + 1]);
-          mma_elem<kBf16>(blk[nt][c], a[i][c][0], a[i][c][1], a[i][c][2], a[i][c][3], b2[2 * i], b2[2 * i + 1]);
-        }
-    }
-  }
+// A pair of float32 numbers as 16-bit ones and what that rounding left.
+template <bool kBf16>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+  hi = Elem<kBf16>::pack(x, y);
+  const float2 back = Elem<kBf16>::unpack(hi);
+  lo = Elem<kBf16>::pack(x - back.x, y - back.y);
 }
 
-// The even split of `total` items over n CTAs: CTA c takes [c, c + 1) * total / n.
-__device__ __forceinline__ int64_t split_at(int64_t c, int64_t total, int64_t n) { return c * total / n; }
-__device__ __forceinline__ int owner(int64_t x, int64_t total, int64_t n) {
-  return static_cast<int>(((x + 1) * n + total - 1) / total - 1);
-}
-
-// Walks the pieces of a CTA's items [x, x_end): a run of one unit's items.
-struct Pieces {
-  int64_t x, x_end, unit_begin;
-  int b, sub;  // sequence; KV head * row_tiles + row tile
-  Seq s;
-  int begin, end;  // items of the unit
-
-  template <class SmemT>
-  __device__ __forceinline__ void load(const AttendParams& p, const SmemT& sm) {
-    const int2 l = b < kLensCached ? sm.lens[b] : load_len(p, b);
-    s = make_seq(p, l.x, l.y);
+// The even split of `total` steps over n workers: the first `rem` take one
+// step more than the others.
+struct Split {
+  uint32_t total, n, each, rem;
+  __device__ __forceinline__ Split(uint32_t total_, uint32_t workers) : total(total_), n(min(workers, total_)) {
+    each = total / n;
+    rem = total - each * n;
   }
-  template <class SmemT>
-  __device__ __forceinline__ void init(const AttendParams& p, const SmemT& sm, int64_t x0, int64_t x1) {
-    x = x0;
-    x_end = x1;
-    b = sm.b0;
-    const int64_t base = (int64_t(sm.base_hi) << 32) | static_cast<uint32_t>(sm.base_lo);
-    load(p, sm);
-    sub = static_cast<int>((x - base) / s.items);
-    unit_begin = base + int64_t(sub) * s.items;
-    begin = end = 0;
-  }
-  // The next piece, or false.
-  template <class SmemT>
-  __device__ __forceinline__ bool next(const AttendParams& p, const SmemT& sm) {
-    if (x >= x_end) return false;
-    if (x == unit_begin + s.items) {
-      unit_begin = x;
-      if (++sub == p.c.n_kv_heads * p.row_tiles) {
-        sub = 0;
-        ++b;
-        load(p, sm);
-      }
-    }
-    begin = static_cast<int>(x - unit_begin);
-    end = static_cast<int>(min(x_end - unit_begin, int64_t(s.items)));
-    x = unit_begin + end;
-    return true;
-  }
-  __device__ __forceinline__ int blocks() const { return s.sink_blocks + s.full - s.win_block; }
-  __device__ __forceinline__ int block_of(int item) const {
-    return item < s.sink_blocks ? item : s.win_block + item - s.sink_blocks;
+  __device__ __forceinline__ uint32_t begin(uint32_t g) const { return g * each + min(g, rem); }
+  __device__ __forceinline__ uint32_t owner(uint32_t x) const {
+    const uint32_t wide = rem * (each + 1);
+    return x < wide ? x / (each + 1) : rem + (x - wide) / each;
   }
 };
 
-template <int kD, int kNT, bool kBf16, bool kInt8>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm)
+template <bool kCg, class T>
+__device__ __forceinline__ T load(const T* p) {
+  if constexpr (kCg) return __ldcg(p);
+  return *p;
+}
+
+// Row `row` of pieces that cover a unit (or a part of it): their sums under a
+// common maximum.  A lane holds one piece's maximum and sum at a time, then
+// kD / 32 columns.  ptr(i): the data of piece i < n, with kCg written by other
+// CTAs (read past the L1).
+template <int kD, int kRows, bool kCg, class Ptr>
+__device__ __forceinline__ void merge_row(int n, int row, int lane, Ptr ptr, float& M, float& L, float (&a)[kD / 32]) {
+  constexpr int kCols = kD / 32;
+  M = -INFINITY;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, load<kCg>(reinterpret_cast<const float2*>(ptr(i)) + row).x);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  const float ref = M == -INFINITY ? 0.f : M;
+  L = 0.f;
+#pragma unroll
+  for (int k = 0; k < kCols; ++k) a[k] = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float w = 0.f;
+    if (i0 + lane < n) {
+      const float2 ml = load<kCg>(reinterpret_cast<const float2*>(ptr(i0 + lane)) + row);
+      w = fast_exp2(ml.x - ref);
+      L += ml.x == -INFINITY ? ml.y : w * ml.y;  // (a row of NaN scores has no maximum; its sum is NaN)
+    }
+    const int cnt = min(32, n - i0);
+#pragma unroll 4
+    for (int j = 0; j < cnt; ++j) {
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const float* src = ptr(i0 + j) + 2 * kRows + row * kD + lane * kCols;
+      if constexpr (kCols == 4) {
+        const float4 x = load<kCg>(reinterpret_cast<const float4*>(src));
+        a[0] += wj * x.x, a[1] += wj * x.y, a[2] += wj * x.z, a[3] += wj * x.w;
+      } else {
+        const float2 x = load<kCg>(reinterpret_cast<const float2*>(src));
+        a[0] += wj * x.x, a[1] += wj * x.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
+}
+
+template <int kD, int kNT, int kR, bool kBf16, bool kInt8>
+__global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
     kv8_attend_kernel(const __grid_constant__ CUtensorMap tm_kc, const __grid_constant__ CUtensorMap tm_vc,
                       const __grid_constant__ CUtensorMap tm_kr, const __grid_constant__ CUtensorMap tm_vr,
                       const AttendParams p) {
   using G = Geo<kD>;
-  using S = Smem<kD, kNT>;
-  constexpr int kStages = S::kStages;
-  constexpr int kChunks = kD / 16;      // 16-wide steps of the head dimension
-  constexpr int kMT = kChunks / kWarps;  // those that a warp accumulates
-  constexpr int kRows = 8 * kNT;
+  using H = Shape<kNT, kR>;
+  using S = Smem<kNT, kR>;
+  constexpr int kWorkers = H::kWorkers, kStages = H::kStages, kRows = H::kRows;
+  constexpr int kChunks = kD / 16;         // 16-wide steps of the head dimension
+  constexpr int kTC = G::kTok / 16;        // 16-token steps of a block step
+  constexpr int kRC = G::kRingTok / 16;    // and of a ring step
+  constexpr int kPiece = kRows * (2 + kD);  // floats of a partial result
   // P as one fp16 number has a relative error of 2^-12, the same as rounding
   // the output to fp16 makes, and far below bf16's.  With fp16 outputs P is
-  // the sum of two fp16 numbers (2^-23); the memory-bound loop has room for it.
+  // the sum of two fp16 numbers (2^-23).
   constexpr bool kSplitP = !kBf16;
-  // Query fragments of 32 rows of 128 would take 64 registers a thread (of 168 that
-  // two CTAs of five warps leave); they are read from shared memory instead.
-  constexpr bool kQShared = kNT * kD >= 256;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   grid_launch_dependents();
   if (smem_u32(smem_raw) & 1023u) {
@@ -378,19 +319,15 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
     return;
   }
   S& sm = *reinterpret_cast<S*>(smem_raw);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&sm.full[s]), 1);
-      mbar_init(smem_u32(&sm.empty[s]), kWarps);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(smem_u32(&sm.q_full[s]), 1);
-      mbar_init(smem_u32(&sm.q_empty[s]), kWarps);
-    }
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const int w = warp / kR, wr = warp % kR;  // worker; its warp
+  if (tid < kWorkers * kStages) {
+    mbar_init(smem_u32(&sm.full[0][0] + tid), 1);
+    mbar_init(smem_u32(&sm.empty[0][0] + tid), kR);
     fence_barrier_init();
   }
-  if (tid == kWarps * 32) {
+  if (tid < 2 * kWorkers) sm.part[tid >> 1][tid & 1].flags = 0;
+  if (tid == H::kThreads - 1) {
     prefetch_tmap(&tm_kc);
     prefetch_tmap(&tm_vc);
     prefetch_tmap(&tm_kr);
@@ -398,608 +335,614 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm)
   }
   grid_dependency_wait();
 
-  // ---- the split: items before each thread's run of sequences
-  const int batch = p.c.batch, per = (batch + kThreads - 1) / kThreads;
+  // ---- the split: steps before each thread's run of sequences
+  const int batch = p.c.batch, per = (batch + H::kThreads - 1) / H::kThreads;
   const int units = p.c.n_kv_heads * p.row_tiles;  // of a sequence
-  int64_t x0, x1, total;
-  {
-    int mine = 0;  // items of this thread's sequences, per unit of them
-    for (int b = tid * per; b < min(batch, (tid + 1) * per); ++b) {
-      const int2 l = load_len(p, b);
-      if (b < kLensCached) sm.lens[b] = l;
-      mine += make_seq(p, l.x, l.y).items;
-    }
-    int before = mine;
-#pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, before, off);
-      if (lane >= off) before += y;
-    }
-    if (lane == 31) sm.scan[warp] = before;
-    __syncthreads();
-    int sum = 0, prior = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w == warp) prior = sum;
-      sum += sm.scan[w];
-    }
-    before += prior - mine;
-    total = int64_t(sum) * units;
-    const int64_t n = min(int64_t(p.n_ctas), total);
-    x0 = split_at(blockIdx.x, total, n);
-    x1 = split_at(blockIdx.x + 1, total, n);
-    if (blockIdx.x >= n) return;  // the same for the whole CTA
-    const int64_t lo = int64_t(before) * units, hi = int64_t(before + mine) * units;
-    if (x0 >= lo && x0 < hi) {
-      int64_t at = lo;
-      for (int b = tid * per;; ++b) {
-        const int2 l = b < kLensCached ? sm.lens[b] : load_len(p, b);
-        const int64_t w = int64_t(make_seq(p, l.x, l.y).items) * units;
-        if (x0 < at + w) {
-          sm.b0 = b;
-          sm.base_hi = static_cast<int>(at >> 32);
-          sm.base_lo = static_cast<int>(at);
-          break;
-        }
-        at += w;
-      }
-    }
-    __syncthreads();
+  int mine = 0;  // steps of this thread's sequences, of one unit
+  for (int b = tid * per; b < min(batch, (tid + 1) * per); ++b) {
+    const int2 l = load_len(p, b);
+    if (b < kLensCached) sm.lens[b] = l;
+    mine += make_seq<kD>(p, l.x, l.y).steps;
   }
-  const int64_t n_split = min(int64_t(p.n_ctas), total);
-
-  Pieces pc;
-  pc.init(p, sm, x0, x1);
-  int qs = 0;
-  uint32_t qphase = 0;
-  uint32_t st = 0, phase = 0;  // stage ring position
-  auto advance = [&]() {
-    if (++st == kStages) st = 0, phase ^= 1;
-  };
-
-  if (warp == kWarps) {
-    // ------------------------------------------------------------- producer
-    bool ok = true;
-    while (ok && pc.next(p, sm)) {
-      if (pc.s.empty) continue;
-      const int h = pc.sub / p.row_tiles, n0 = (pc.sub % p.row_tiles) * kRowTile;
-      // queries: one row a lane
-      if (lane == 0) ok = mbar_wait(smem_u32(&sm.q_empty[qs]), qphase ^ 1, p.err);
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      if (!ok) break;
-      const int n_rows = min(kRows, p.rows - n0);
-      const uint32_t qb = smem_u32(&sm.q_full[qs]);
-      if (lane == 0) mbar_arrive_expect_tx(qb, n_rows * kD * 2);
-      __syncwarp();
-      if (lane < n_rows) {
-        const int n = n0 + lane, t = n / p.group;
-        bulk_load(smem_u32(sm.q[qs][lane]), p.q.row(pc.b, h * p.group + n - t * p.group, t), kD * 2, qb);
-      }
-      if (++qs == 2) qs = 0, qphase ^= 1;
-
-      const int blocks = pc.blocks();
-      for (int i0 = pc.begin; ok && i0 < min(pc.end, blocks); i0 += 32) {
-        int page = 0;
-        float2 sc = make_float2(NAN, NAN);
-        if (i0 + lane < min(pc.end, blocks)) {  // 32 items' page numbers and scales at once
-          page = __ldg(p.c.page_table + int64_t(pc.b) * p.c.max_blocks + pc.block_of(i0 + lane));
-          if (page >= 0 && page < p.c.n_pages) {
-            sc = __ldg(p.c.scales + int64_t(page) * p.c.n_kv_heads + h);
-          } else {
-            set_error(p.err, NSA_ERR_INVALID);
-            page = 0;
-          }
-        }
-        const int cnt = min(32, min(pc.end, blocks) - i0);
-        for (int j = 0; j < cnt; ++j) {
-          const int pg = __shfl_sync(0xffffffffu, page, j);
-          const float2 s2 = make_float2(__shfl_sync(0xffffffffu, sc.x, j), __shfl_sync(0xffffffffu, sc.y, j));
-          if (lane == 0) {
-            ok = mbar_wait(smem_u32(&sm.empty[st]), phase ^ 1, p.err);
-            if (ok) {
-              const uint32_t fb = smem_u32(&sm.full[st]), dst = smem_u32(sm.stage[st]);
-              sm.scale[st] = s2;  // published by the arrive
-              mbar_arrive_expect_tx(fb, G::kStageBytes);
-              const int row = (pg * p.c.n_kv_heads + h) * kBlock;
-              tma_load_2d(dst, &tm_kc, fb, 0, row);
-              tma_load_2d(dst + G::kCodeBytes, &tm_vc, fb, 0, row);
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          advance();
-        }
-      }
-      if (ok && pc.end > blocks && pc.s.len % kBlock) {  // the incomplete block: 32 ring slots a stage
-        const int tail = pc.s.len % kBlock, slot0 = (pc.s.full * kBlock) % kRing;
-        const int unit = pc.b * p.c.n_kv_heads + h;
-        for (int f = 0; f < tail; f += 32) {
-          if (lane == 0) {
-            ok = mbar_wait(smem_u32(&sm.empty[st]), phase ^ 1, p.err);
-            if (ok) {
-              const uint32_t fb = smem_u32(&sm.full[st]), dst = smem_u32(sm.stage[st]);
-              const int boxes = min(4, (tail - f + 7) / 8);  // 8 rows each, only those that hold tokens
-              mbar_arrive_expect_tx(fb, boxes * 8 * kD * 4);
-              for (int r = 0; r < boxes; ++r)
-                for (uint32_t c = 0; c < G::kRegions; ++c) {
-                  const uint32_t d = dst + c * G::kRegion + r * 1024;
-                  tma_load_2d(d, &tm_kr, fb, c * 64, unit * kRing + slot0 + f + 8 * r);
-                  tma_load_2d(d + G::kCodeBytes, &tm_vr, fb, c * 64, unit * kRing + slot0 + f + 8 * r);
-                }
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
-          advance();
-        }
-      }
-    }
+  int before = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += y;
+  }
+  if (lane == 31) sm.scan[warp] = before;
+  __syncthreads();
+  int sum = 0, prior = 0;
+#pragma unroll
+  for (int i = 0; i < H::kWarps; ++i) {
+    if (i == warp) prior = sum;
+    sum += sm.scan[i];
+  }
+  if (int64_t(sum) * units > 0x7fffffff) {  // (16 TB of codes)
+    if (tid == 0) set_error(p.err, NSA_ERR_INVALID);
     return;
   }
+  const Split split(static_cast<uint32_t>(sum) * units, gridDim.x * kWorkers);
+  if (blockIdx.x * kWorkers >= split.n) return;  // the whole CTA has nothing to do
+  const uint32_t worker = blockIdx.x * kWorkers + w;
+  const uint32_t x0 = worker < split.n ? split.begin(worker) : split.total;
+  const int n_steps = worker < split.n ? static_cast<int>(split.begin(worker + 1) - x0) : 0;
+  sm.before[tid] = before + prior - mine;
+  __syncthreads();
 
-  // -------------------------------------------------------------- consumers
-  // After a wait that ran out (the error word is set) a warp waits no more but
-  // keeps its schedule of named barriers, so that no other warp waits for it.
-  const int g = lane >> 2, t = lane & 3;
-  bool aborted = false;
-  uint32_t qf[kQShared ? 1 : kNT][kChunks][2];
-  float qscale[kNT][2];  // of rows 8nt + 2t, 8nt + 2t + 1: the row's power of two, sm_scale and log2(e)
-  float m[kNT][2], l[kNT][2];
-  float acc[kNT][kMT][4];  // dims 16c + 2g (0, 1) and 16c + 2g + 1 (2, 3), rows 2t (0, 2) and 2t + 1 (1, 3)
-
-  while (pc.next(p, sm)) {
-    const int h = pc.sub / p.row_tiles, n0 = (pc.sub % p.row_tiles) * kRowTile;
-    const Seq s = pc.s;
-    const bool nothing = pc.s.empty;
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) m[nt][e] = -INFINITY, l[nt][e] = 0.f;
-#pragma unroll
-      for (int c = 0; c < kMT; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[nt][c][e] = 0.f;
+  // ---- issuing (a worker's first warp): lane i knows step batch0 + i
+  int cur_b = 0, batch0 = -32, issued = 0;
+  int cur_rel = 0;  // first step of sequence cur_b, from the worker's first
+  uint32_t i_st = 0, i_ph = 0;
+  Step mystep{};
+  int myrow = 0;
+  if (wr == 0 && n_steps > 0) {  // the sequence of the first step: the last one that begins at it or before
+    const int at = static_cast<int>(x0 / units), threads = (batch + per - 1) / per;
+    int n = 0;
+    for (int i = lane; i < threads; i += 32) n += sm.before[i] <= at;
+    n = __reduce_add_sync(0xffffffffu, n) - 1;
+    cur_b = n * per;
+    int begin = sm.before[n];
+    for (;;) {
+      const int2 l = cur_b < kLensCached ? sm.lens[cur_b] : load_len(p, cur_b);
+      const int steps = make_seq<kD>(p, l.x, l.y).steps;
+      if (at < begin + steps) break;
+      begin += steps;
+      ++cur_b;
     }
-    int limit[kNT][2];  // positions below it are seen
-    const int first_pos = s.len - s.cnt + 1;
-    auto limit_of = [&](int n) { return max(first_pos + min(min(n, p.rows - 1) / p.group, s.cnt - 1), 0); };
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) limit[nt][e] = limit_of(n0 + 8 * nt + 2 * t + e);
-    const int limit_min = limit_of(n0), limit_max = limit_of(n0 + kRows - 1);
+    cur_rel = begin * units - static_cast<int>(x0);
+  }
+  auto head_of = [&](int sub) { return p.row_tiles == 1 ? sub : sub / p.row_tiles; };
+  auto limit_at = [&](int len, int cnt, int n) {
+    return max(len - cnt + 1 + min(token_of(p, min(n, p.rows - 1)), cnt - 1), 0);
+  };
+  auto fetch = [&](int k0) {
+    batch0 = k0;
+    const int k = k0 + lane, k_end = min(k0 + 32, n_steps);
+    bool found = k >= n_steps;
+    Seq s;
+    int step = 0, sub = 0, b = 0;
+    for (;;) {
+      const int2 l = cur_b < kLensCached ? sm.lens[cur_b] : load_len(p, cur_b);
+      const Seq c = make_seq<kD>(p, l.x, l.y);
+      const int end = cur_rel + c.steps * units;
+      if (!found && k < end) {
+        const uint32_t off = static_cast<uint32_t>(k - cur_rel);
+        sub = off / static_cast<uint32_t>(c.steps);
+        step = off - sub * c.steps;
+        b = cur_b;
+        s = c;
+        found = true;
+      }
+      if (k_end <= end) break;
+      ++cur_b;
+      cur_rel = end;
+    }
+    if (k >= n_steps) return;
+    const int h = head_of(sub), n0 = (sub - h * p.row_tiles) * kRows;
+    mystep.b = b;
+    mystep.sub = sub;
+    mystep.len = s.len;
+    mystep.cnt = s.cnt;
+    mystep.step = step;
+    mystep.steps = s.steps;
+    mystep.pos0 = 0;
+    mystep.ks = mystep.vs = 1.f;
+    int flags = (step == 0 ? kBegin | kFirst : 0) | (step == s.steps - 1 ? kEnd | kLast : 0);
+    flags |= (k == 0 ? kFirst : 0) | (k == n_steps - 1 ? kLast : 0);
+    const int block_steps = (s.sink_blocks + s.full - s.win_block) * G::kSteps;
+    if (s.empty) {
+      flags |= kEmpty;
+    } else if (step < block_steps) {
+      const int item = step / G::kSteps, tok = (step % G::kSteps) * G::kTok;
+      const int block = item < s.sink_blocks ? item : s.win_block + item - s.sink_blocks;
+      int page = __ldg(p.c.page_table + int64_t(b) * p.c.max_blocks + block);
+      float2 sc = make_float2(NAN, NAN);
+      if (page >= 0 && page < p.c.n_pages) {
+        sc = __ldg(p.c.scales + int64_t(page) * p.c.n_kv_heads + h);
+      } else {
+        set_error(p.err, NSA_ERR_INVALID);
+        page = 0;
+      }
+      mystep.ks = sc.x;
+      mystep.vs = sc.y;
+      mystep.pos0 = block * kBlock + tok;
+      myrow = (page * p.c.n_kv_heads + h) * kBlock + tok;
+      const int lo = limit_at(s.len, s.cnt, n0), hi = limit_at(s.len, s.cnt, n0 + kRows - 1);
+      if (mystep.pos0 + G::kTok > lo ||
+          (p.window >= 0 && mystep.pos0 < hi - p.window && mystep.pos0 + G::kTok > p.sink))
+        flags |= kMasked;
+    } else {
+      mystep.pos0 = s.full * kBlock + (step - block_steps) * G::kRingTok;
+      myrow = (b * p.c.n_kv_heads + h) * kRing + mystep.pos0 % kRing;
+      flags |= kRingStep | kMasked | (min(G::kRingTok, s.len - mystep.pos0) << 8);
+    }
+    mystep.flags = flags;
+  };
+  bool aborted = false;
+  auto issue_to = [&](int upto) {  // stages steps [issued, upto)
+    for (upto = min(upto, n_steps); issued < upto; ++issued) {
+      if (issued >= batch0 + 32) fetch(issued);
+      if (lane == issued - batch0 && !aborted) {
+        if (kR > 1 && !mbar_wait(smem_u32(&sm.empty[w][i_st]), i_ph ^ 1, p.err)) {
+          aborted = true;
+        } else {
+          const uint32_t fb = smem_u32(&sm.full[w][i_st]), dst = smem_u32(sm.stage[w][i_st]);
+          if (mystep.flags & kEmpty) {
+            sm.step[w][i_st] = mystep;
+            mbar_arrive(fb);
+          } else if (!(mystep.flags & kRingStep)) {
+            // the copies before the scales have arrived: the phase ends with the arrive below
+            tma_load_2d(dst, &tm_kc, fb, 0, myrow);
+            tma_load_2d(dst + kHalf, &tm_vc, fb, 0, myrow);
+            sm.step[w][i_st] = mystep;
+            mbar_arrive_expect_tx(fb, kStageBytes);
+          } else {
+            const int boxes = ((mystep.flags >> 8) + 7) / 8;  // of 8 slots, those that hold tokens
+            sm.step[w][i_st] = mystep;
+            mbar_arrive_expect_tx(fb, boxes * 8 * kD * 4);
+            for (int r = 0; r < boxes; ++r)
+              for (uint32_t c = 0; c < G::kRegions; ++c) {
+                tma_load_2d(dst + c * G::kRegion + r * 1024, &tm_kr, fb, c * 64, myrow + 8 * r);
+                tma_load_2d(dst + kHalf + c * G::kRegion + r * 1024, &tm_vr, fb, c * 64, myrow + 8 * r);
+              }
+          }
+        }
+      }
+      if (++i_st == kStages) i_st = 0, i_ph ^= 1;
+    }
+    __syncwarp();
+  };
+  if (wr == 0) issue_to(kStages);
 
-    if (!nothing) {
-      // ---- queries: fp16 fragments, k index permuted as the codes' ldmatrix gives it
-      if (!aborted && !mbar_wait(smem_u32(&sm.q_full[qs]), qphase, p.err)) aborted = true;
+  // ---- the worker's steps.  After a wait that ran out (the error word is
+  // set) a warp waits no more, so that it still reaches the CTA's barriers.
+  uint32_t qf[kNT][kChunks][2];
+  float qscale[kNT][2];  // of rows 8nt + 2t + (0, 1): the row's power of two, sm_scale and log2(e)
+  float m[kNT][2], l[kNT][2];
+  int limit[kNT][2];           // positions below it are seen
+  float acc[kNT][kChunks][4];  // dims 16c + 2g (0, 1) and 16c + 2g + 1 (2, 3), rows 2t (0, 2) and 2t + 1 (1, 3)
+  bool begins = false;         // the piece holds its unit's first step
+  uint32_t st = 0, ph = 0;
+  for (int k = 0; k < n_steps; ++k) {
+    if (!aborted && !mbar_wait(smem_u32(&sm.full[w][st]), ph, p.err)) aborted = true;
+    aborted = __any_sync(0xffffffffu, aborted);
+    const Step s = sm.step[w][st];
+    const bool ring = s.flags & kRingStep, empty = s.flags & kEmpty;
+    const int h = head_of(s.sub), n0 = (s.sub - h * p.row_tiles) * kRows + 8 * kNT * wr;  // this warp's rows
+    if (s.flags & kFirst) {
+      begins = s.flags & kBegin;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        if (kQShared && nt != warp) continue;  // each warp converts 8 rows for all
-        uint2 raw[kChunks];
-        float top = 0.f;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          raw[c] = *reinterpret_cast<const uint2*>(&sm.q[qs][8 * nt + g][32 * c + 8 * t]);
-          const float2 a = Elem<kBf16>::unpack(raw[c].x), b = Elem<kBf16>::unpack(raw[c].y);
-          top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
+        for (int e = 0; e < 2; ++e) {
+          m[nt][e] = -INFINITY, l[nt][e] = 0.f;
+          limit[nt][e] = limit_at(s.len, s.cnt, n0 + 8 * nt + 2 * t + e);
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // a power of two from the exponent field; rows of zeros or infinities as they are
-        int ex = static_cast<int>(__float_as_uint(top) >> 23);
-        ex = (top == 0.f || ex == 255) ? 127 : min(max(ex, 1), 253);
-        const float f = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
-        const float back = __uint_as_float(static_cast<uint32_t>(ex) << 23) * p.scale_log2;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const float2 a = Elem<kBf16>::unpack(raw[c].x), b = Elem<kBf16>::unpack(raw[c].y);
-          const uint32_t lo = pack_half2(a.x * f, a.y * f), hi = pack_half2(b.x * f, b.y * f);
-          if constexpr (kQShared)
-            *reinterpret_cast<uint2*>(&sm.q[qs][8 * nt + g][32 * c + 8 * t]) = make_uint2(lo, hi);
-          else
-            qf[nt][c][0] = lo, qf[nt][c][1] = hi;
-        }
-        if constexpr (kQShared) {
-          if (t == 0) sm.q_scale[8 * nt + g] = back;
-        } else {
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[nt][c][e] = 0.f;
+      }
+      if (!empty) {
+        // queries: fp16 fragments, k index permuted as the codes' ldmatrix gives it
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          const int n = min(n0 + 8 * nt + g, p.rows - 1), tok = token_of(p, n);
+          const uint16_t* row = p.q.row(s.b, h * p.group + n - tok * p.group, tok) + 4 * t;
+          uint2 raw[kChunks];
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) raw[c] = __ldg(reinterpret_cast<const uint2*>(row + 16 * c));
+          float top = 0.f;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            const float2 a = Elem<kBf16>::unpack(raw[c].x), b = Elem<kBf16>::unpack(raw[c].y);
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
+          }
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          // a power of two from the exponent field; rows of zeros or infinities as they are
+          int ex = static_cast<int>(__float_as_uint(top) >> 23);
+          ex = (top == 0.f || ex == 255) ? 127 : min(max(ex, 1), 253);
+          const float f = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+          const float back = __uint_as_float(static_cast<uint32_t>(ex) << 23) * p.scale_log2;
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            const float2 a = Elem<kBf16>::unpack(raw[c].x), b = Elem<kBf16>::unpack(raw[c].y);
+            qf[nt][c][0] = pack_half2(a.x * f, a.y * f);
+            qf[nt][c][1] = pack_half2(b.x * f, b.y * f);
+          }
           qscale[nt][0] = __shfl_sync(0xffffffffu, back, 8 * t);      // from a lane of row 2t
           qscale[nt][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);  // and of 2t + 1
         }
       }
-      if constexpr (kQShared) {
-        sync_consumers();
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-          const float2 x = *reinterpret_cast<const float2*>(&sm.q_scale[8 * nt + 2 * t]);
-          qscale[nt][0] = x.x, qscale[nt][1] = x.y;
-        }
-      } else {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sm.q_empty[qs]));
-        if (++qs == 2) qs = 0, qphase ^= 1;
-      }
     }
-    const uint32_t q_at = smem_u32(&sm.q[qs][g][8 * t]);  // kQShared: this lane's fragments
-    auto q_frag = [&](int nt, int c, uint32_t& b0, uint32_t& b1) {
-      if constexpr (kQShared)
-        lds8(q_at + nt * 8 * G::kQStride + 32 * c, b0, b1);
-      else
-        b0 = qf[nt][c][0], b1 = qf[nt][c][1];
-    };
 
-    const int blocks = pc.blocks();
-    for (int item = pc.begin; !nothing && item < pc.end; ++item) {
-      const bool ring = item >= blocks;  // the incomplete block
-      const int pos0 = (ring ? s.full : pc.block_of(item)) * kBlock;
-      const int tail = s.len - s.full * kBlock;  // its tokens
-      const int stages = ring && tail > 32 ? 2 : 1;
-      uint32_t st1 = st + 1, phase1 = phase;  // the second stage of an incomplete block
-      if (st1 == kStages) st1 = 0, phase1 ^= 1;
-      if (!aborted && !mbar_wait(smem_u32(&sm.full[st]), phase, p.err)) aborted = true;
-      if (stages == 2 && !aborted && !mbar_wait(smem_u32(&sm.full[st1]), phase1, p.err)) aborted = true;
-
-      // ---- scores of this warp's 16 tokens, S^T: token g (0, 1), g + 8 (2, 3); rows 2t, 2t + 1
-      float sc[kNT][4];
+    if (!empty) {
+      const uint32_t kb = smem_u32(sm.stage[w][st]), vb = kb + kHalf;
+      // ---- scores, S^T: token g (0, 1), g + 8 (2, 3); rows 2t, 2t + 1
+      float sc[kTC][kNT][4];
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+      for (int i = 0; i < kTC; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) sc[nt][e] = 0.f;
-      float vs = 1.f;
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][nt][e] = 0.f;
       if (!ring) {
-        const float2 scale = sm.scale[st];
-        vs = scale.y;
-        const uint32_t kb = smem_u32(sm.stage[st]);
-        const uint32_t row = 16 * warp + ((lane >> 3) & 1) * 8 + (lane & 7), hi = lane >> 4;
 #pragma unroll
-        for (int c = 0; c < kChunks; c += 2) {
-          uint32_t r[4];
-          const uint32_t chunk = kD == 128 ? ((c + hi) ^ (row & 7)) : ((c + hi) ^ ((row >> 1) & 3));
-          ldmatrix_x4(kb + row * kD + chunk * 16, r[0], r[1], r[2], r[3]);
+        for (int c = 0; c < kChunks; c += 2)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < kTC; ++i) {
+            const uint32_t row = 16 * i + ((lane >> 3) & 1) * 8 + (lane & 7);
+            const uint32_t chunk = (c + (lane >> 4)) ^ (kD == 128 ? (row & 7) : ((row >> 1) & 3));
+            uint32_t r[4];
+            ldmatrix_x4(kb + row * kD + chunk * 16, r[0], r[1], r[2], r[3]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t a0, a1, a2, a3;
+              to_half<kInt8, false>(r[2 * j], a0, a2);
+              to_half<kInt8, false>(r[2 * j + 1], a1, a3);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt)
+                mma_16816(sc[i][nt], a0, a1, a2, a3, qf[nt][c + j][0], qf[nt][c + j][1]);
+            }
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRC; ++i)
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            // row & 7 == g for both of this lane's rows
+            const uint32_t at = kb + (c >> 2) * G::kRegion + (16 * i + g) * 128 +
+                                ((((c & 3) * 2 + (t >> 1)) ^ g) << 4) + (t & 1) * 8;
             uint32_t a0, a1, a2, a3;
-            to_half<kInt8, false>(r[2 * i], a0, a2);
-            to_half<kInt8, false>(r[2 * i + 1], a1, a3);
+            lds8(at, a0, a2);
+            lds8(at + 8 * 128, a1, a3);
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt) {
-              uint32_t b0, b1;
-              q_frag(nt, c + i, b0, b1);
-              mma_16816(sc[nt], a0, a1, a2, a3, b0, b1);
+              uint32_t b0 = qf[nt][c][0], b1 = qf[nt][c][1];
+              if constexpr (kBf16) b0 = half_to_bf16(b0), b1 = half_to_bf16(b1);
+              mma_elem<kBf16>(sc[i][nt], a0, a1, a2, a3, b0, b1);
             }
           }
-        }
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[nt][e] *= scale.x * qscale[nt][e & 1];
-      } else if (16 * warp < tail) {
-        const uint32_t kb = smem_u32(sm.stage[warp < 2 ? st : st1]);
-        const uint32_t row = 16 * (warp & 1) + g;  // row & 7 == g for both of this lane's rows
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          const uint32_t at = kb + (c >> 2) * G::kRegion + ((((c & 3) * 2 + (t >> 1)) ^ g) << 4) + (t & 1) * 8;
-          uint32_t a0, a1, a2, a3;
-          lds8(at + row * 128, a0, a2);
-          lds8(at + (row + 8) * 128, a1, a3);
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            uint32_t b0, b1;
-            q_frag(nt, c, b0, b1);
-            if constexpr (kBf16) b0 = half_to_bf16(b0), b1 = half_to_bf16(b1);
-            mma_elem<kBf16>(sc[nt], a0, a1, a2, a3, b0, b1);
-          }
-        }
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[nt][e] *= qscale[nt][e & 1];
       }
-      // ---- masks, where an edge crosses the block
-      const bool masked = ring || pos0 + kBlock > limit_min ||
-                          (p.window >= 0 && pos0 < limit_max - p.window && pos0 + kBlock > p.sink);
-      if (masked) {
-#pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int pos = pos0 + 16 * warp + g + (e >> 1) * 8, lim = limit[nt][e & 1];
-            if (!sees(p, pos, lim)) sc[nt][e] = -INFINITY;
-          }
-      }
-      // ---- rows' maxima over the 64 tokens
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        float a = fmaxf(sc[nt][0], sc[nt][2]), b = fmaxf(sc[nt][1], sc[nt][3]);
+        const float f0 = s.ks * qscale[nt][0], f1 = s.ks * qscale[nt][1];
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, off));
-          b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, off));
-        }
-        if (g == 0) *reinterpret_cast<float2*>(&sm.mx[warp][8 * nt + 2 * t]) = make_float2(a, b);
+        for (int i = 0; i < kTC; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][nt][e] *= (e & 1) ? f1 : f0;
       }
-      sync_consumers();
-      float row_vs[kNT][2];
+      if (s.flags & kMasked) {
+#pragma unroll
+        for (int i = 0; i < kTC; ++i)
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if ((ring && i >= kRC) || !sees(p, s.pos0 + 16 * i + g + (e >> 1) * 8, limit[nt][e & 1]))
+                sc[i][nt][e] = -INFINITY;
+      }
+      // ---- online softmax, and P as B fragments
+      float alpha[kNT][2], row_vs[kNT][2];
+      uint32_t pb[kTC][kNT][2], pl[kTC][kNT][2];
       bool moved = false;
-      float alpha[kNT][2];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        float2 top = *reinterpret_cast<const float2*>(&sm.mx[0][8 * nt + 2 * t]);
-#pragma unroll
-        for (int w = 1; w < kWarps; ++w) {
-          const float2 o = *reinterpret_cast<const float2*>(&sm.mx[w][8 * nt + 2 * t]);
-          top.x = fmaxf(top.x, o.x);
-          top.y = fmaxf(top.y, o.y);
-        }
-        const float tops[2] = {top.x, top.y};
+        float ref[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+          float x = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kTC; ++i) x = fmaxf(x, fmaxf(sc[i][nt][e], sc[i][nt][2 + e]));
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
           // a row that sees nothing of this block takes nothing of it, not even a scale that is NaN
-          row_vs[nt][e] = tops[e] == -INFINITY ? 0.f : vs;
-          const float mn = fmaxf(m[nt][e], tops[e]);
-          const float ref = mn == -INFINITY ? 0.f : mn;
-          alpha[nt][e] = fast_exp2(m[nt][e] - ref);
+          row_vs[nt][e] = x == -INFINITY ? 0.f : s.vs;
+          const float mn = fmaxf(m[nt][e], x);
+          ref[e] = mn == -INFINITY ? 0.f : mn;
+          alpha[nt][e] = fast_exp2(m[nt][e] - ref[e]);
           moved |= alpha[nt][e] != 1.f;
           m[nt][e] = mn;
-          const float p0 = fast_exp2(sc[nt][e] - ref), p1 = fast_exp2(sc[nt][2 + e] - ref);
-          l[nt][e] = l[nt][e] * alpha[nt][e] + (p0 + p1);
-          // P[row][token], 16-bit, in one or two parts
-          const uint32_t at = (8 * nt + 2 * t + e) * kPStride + (16 * warp + g) * 2;
+          l[nt][e] *= alpha[nt][e];
+        }
+#pragma unroll
+        for (int i = 0; i < kTC; ++i) {
+          const float p0 = fast_exp2(sc[i][nt][0] - ref[0]), p1 = fast_exp2(sc[i][nt][1] - ref[1]);
+          const float p2 = fast_exp2(sc[i][nt][2] - ref[0]), p3 = fast_exp2(sc[i][nt][3] - ref[1]);
+          l[nt][0] += p0 + p2;
+          l[nt][1] += p1 + p3;
+          uint32_t lo0 = 0, lo1 = 0;
           if (kBf16 && ring) {
-            store_p<true>(sm, at, p0, true);
-            store_p<true>(sm, at + 16, p1, true);
+            split_pair<true>(p0, p1, pb[i][nt][0], lo0);
+            split_pair<true>(p2, p3, pb[i][nt][1], lo1);
+          } else if (kSplitP) {
+            split_pair<false>(p0, p1, pb[i][nt][0], lo0);
+            split_pair<false>(p2, p3, pb[i][nt][1], lo1);
           } else {
-            store_p<false>(sm, at, p0, kSplitP);
-            store_p<false>(sm, at + 16, p1, kSplitP);
+            pb[i][nt][0] = pack_half2(p0, p1);
+            pb[i][nt][1] = pack_half2(p2, p3);
+          }
+          pb[i][nt][0] = movmatrix_trans(pb[i][nt][0]);  // tokens 2t, 2t + 1 of row g
+          pb[i][nt][1] = movmatrix_trans(pb[i][nt][1]);  // and 2t + 8, 2t + 9
+          if (kSplitP || ring) {
+            pl[i][nt][0] = movmatrix_trans(lo0);
+            pl[i][nt][1] = movmatrix_trans(lo1);
           }
         }
       }
-      sync_consumers();
-
-      // ---- this warp's head dimensions: O^T += V^T P^T over the 64 tokens
-      float blk[kNT][kMT][4];
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-        for (int c = 0; c < kMT; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) blk[nt][c][e] = 0.f;
-      const uint32_t pa = ((lane & 7) * kPStride) + (lane >> 3) * 16;  // ldmatrix: 8 rows of P, 32 tokens
-      const uint32_t ph = smem_u32(sm.p_hi) + pa, pl = smem_u32(sm.p_lo) + pa;
-      if (!ring) {
-        const uint32_t vb = smem_u32(sm.stage[st]) + G::kCodeBytes;
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {  // 32 tokens
-          uint32_t a[2][kMT][4];          // [16 tokens][chunk]
-          if constexpr (kMT == 2) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const uint32_t row = 32 * kk + 16 * i + ((lane >> 3) & 1) * 8 + (lane & 7);
-              const uint32_t chunk = (2 * warp + (lane >> 4)) ^ (row & 7);
-              uint32_t r[4];
-              ldmatrix_x4_trans(vb + row * kD + chunk * 16, r[0], r[1], r[2], r[3]);
-#pragma unroll
-              for (int c = 0; c < 2; ++c) {
-                to_half<kInt8, true>(r[2 * c], a[i][c][0], a[i][c][1]);
-                to_half<kInt8, true>(r[2 * c + 1], a[i][c][2], a[i][c][3]);
-              }
-            }
-          } else {
-            const uint32_t row = 32 * kk + lane;
-            const uint32_t chunk = warp ^ ((row >> 1) & 3);
-            uint32_t r[4];
-            ldmatrix_x4_trans(vb + row * kD + chunk * 16, r[0], r[1], r[2], r[3]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              to_half<kInt8, true>(r[2 * i], a[i][0][0], a[i][0][1]);
-              to_half<kInt8, true>(r[2 * i + 1], a[i][0][2], a[i][0][3]);
-            }
-          }
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            uint32_t b[4];
-            ldmatrix_x4(ph + nt * 8 * kPStride + kk * 64, b[0], b[1], b[2], b[3]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-              for (int c = 0; c < kMT; ++c)
-                mma_16816(blk[nt][c], a[i][c][0], a[i][c][1], a[i][c][2], a[i][c][3], b[2 * i], b[2 * i + 1]);
-            if constexpr (kSplitP) {
-              ldmatrix_x4(pl + nt * 8 * kPStride + kk * 64, b[0], b[1], b[2], b[3]);
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int c = 0; c < kMT; ++c)
-                  mma_16816(blk[nt][c], a[i][c][0], a[i][c][1], a[i][c][2], a[i][c][3], b[2 * i], b[2 * i + 1]);
-            }
-          }
-        }
-      } else {
-        ring_values<kD, kNT, kBf16>(sm, p, st, st1, tail, pos0, warp, lane, limit_of, n0, ph, pl, blk);
-      }
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&sm.empty[st]));
-        if (stages == 2) mbar_arrive(smem_u32(&sm.empty[st1]));
-      }
-      advance();
-      if (stages == 2) advance();
       if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-          for (int c = 0; c < kMT; ++c)
+          for (int c = 0; c < kChunks; ++c)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[nt][c][e] *= alpha[nt][e & 1];
       }
+      // ---- O^T += vs V^T P^T
+      if (!ring) {
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+        for (int c = 0; c < kChunks; c += 2) {
+          float blk[2][kNT][4];
 #pragma unroll
-        for (int c = 0; c < kMT; ++c)
+          for (int j = 0; j < 2; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[nt][c][e] += row_vs[nt][e & 1] * blk[nt][c][e];
-    }
-
-    if (kQShared && !nothing) {  // the slot was written by plain stores; a bulk copy may follow
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sm.q_empty[qs]));
-      if (++qs == 2) qs = 0, qphase ^= 1;
-    }
-
-    // ---- end of the piece: the rows' sums over lanes and warps
-    float2 sum[kNT];
+            for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      float a = l[nt][0], b = l[nt][1];
+              for (int e = 0; e < 4; ++e) blk[j][nt][e] = 0.f;
 #pragma unroll
-      for (int off = 4; off < 32; off <<= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, off);
-        b += __shfl_xor_sync(0xffffffffu, b, off);
+          for (int i = 0; i < kTC; ++i) {
+            const uint32_t row = 16 * i + ((lane >> 3) & 1) * 8 + (lane & 7);
+            const uint32_t chunk = (c + (lane >> 4)) ^ (kD == 128 ? (row & 7) : ((row >> 1) & 3));
+            uint32_t r[4];
+            ldmatrix_x4_trans(vb + row * kD + chunk * 16, r[0], r[1], r[2], r[3]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              uint32_t a0, a1, a2, a3;
+              to_half<kInt8, true>(r[2 * j], a0, a1);
+              to_half<kInt8, true>(r[2 * j + 1], a2, a3);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                mma_16816(blk[j][nt], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
+                if constexpr (kSplitP) mma_16816(blk[j][nt], a0, a1, a2, a3, pl[i][nt][0], pl[i][nt][1]);
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[nt][c + j][e] += row_vs[nt][e & 1] * blk[j][nt][e];
+        }
+      } else {
+        const int n_tok = s.flags >> 8;
+        for (int i = 0; i < kRC && 16 * i < n_tok; ++i) {
+          // (selects instead of a variable index: the fragments stay in registers)
+          uint32_t b0[kNT], b1[kNT], c0[kNT], c1[kNT];
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            b0[nt] = i ? pb[kRC - 1][nt][0] : pb[0][nt][0], b1[nt] = i ? pb[kRC - 1][nt][1] : pb[0][nt][1];
+            c0[nt] = i ? pl[kRC - 1][nt][0] : pl[0][nt][0], c1[nt] = i ? pl[kRC - 1][nt][1] : pl[0][nt][1];
+          }
+#pragma unroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t v[4], a[4], bad = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9: dims 2g, 2g + 1
+              const uint32_t row = 16 * i + 2 * t + (e & 1) + (e >> 1) * 8;
+              v[e] = lds4(vb + (c >> 2) * G::kRegion + row * 128 + ((((c & 3) * 2 + (g >> 2)) ^ (row & 7)) << 4) +
+                          (g & 3) * 4);
+              if (static_cast<int>(row) >= n_tok) v[e] = 0u;  // no token: whatever the slot held
+              bad |= nonfinite_mask<kBf16>(v[e]);
+            }
+            a[0] = __byte_perm(v[0], v[1], 0x5410);
+            a[1] = __byte_perm(v[0], v[1], 0x7632);
+            a[2] = __byte_perm(v[2], v[3], 0x5410);
+            a[3] = __byte_perm(v[2], v[3], 0x7632);
+            if (__any_sync(0xffffffffu, bad != 0)) {
+              // Values that are not finite would reach rows that do not see
+              // them (0 * NaN).  They are taken out, and a product of their
+              // places with the rows' masks says which sums they make NaN.
+              const uint32_t one = kBf16 ? 0x3f803f80u : 0x3c003c00u;
+              uint32_t at[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t mk = nonfinite_mask<kBf16>(a[e]);
+                at[e] = one & mk;
+                a[e] &= ~mk;
+              }
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                const int lim = limit_at(s.len, s.cnt, n0 + 8 * nt + g);
+                uint32_t see[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int pos = s.pos0 + 16 * i + 2 * t + 8 * e;
+                  see[e] = one & ((sees(p, pos, lim) ? 0xffffu : 0u) | (sees(p, pos + 1, lim) ? 0xffff0000u : 0u));
+                }
+                float hit[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_elem<kBf16>(hit, at[0], at[1], at[2], at[3], see[0], see[1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (hit[e] > 0.f) acc[nt][c][e] = NAN;
+              }
+            }
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt) {
+              mma_elem<kBf16>(acc[nt][c], a[0], a[1], a[2], a[3], b0[nt], b1[nt]);
+              mma_elem<kBf16>(acc[nt][c], a[0], a[1], a[2], a[3], c0[nt], c1[nt]);
+            }
+          }
+        }
       }
-      sum[nt] = make_float2(a, b);
     }
-    sync_consumers();  // the maxima of the last item have been read
-    if (g == 0) {
+    __syncwarp();
+    if (kR > 1 && lane == 0) mbar_arrive(smem_u32(&sm.empty[w][st]));
+    if (++st == kStages) st = 0, ph ^= 1;
+    // one warp refills the stage it has just read; with several, the one before,
+    // which the others have most likely left
+    if (wr == 0) issue_to(kR == 1 ? k + 1 + kStages : k + kStages);
+
+    if (!(s.flags & kLast)) continue;
+    // ---- end of the piece
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) *reinterpret_cast<float2*>(&sm.mx[warp][8 * nt + 2 * t]) = sum[nt];
-    }
-    sync_consumers();
+    for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      sum[nt] = make_float2(0.f, 0.f);
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float2 o = *reinterpret_cast<const float2*>(&sm.mx[w][8 * nt + 2 * t]);
-        sum[nt].x += o.x;
-        sum[nt].y += o.y;
-      }
-    }
-    const bool whole = pc.begin == 0 && pc.end == s.items;
-    if (whole) {
+        for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
+    if (begins && (s.flags & kEnd)) {
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int n = n0 + 8 * nt + 2 * t + e;
           if (n >= p.rows) continue;
-          const int tok = n / p.group;
-          const float L = e ? sum[nt].y : sum[nt].x;
-          const float inv = (L == 0.f || tok >= s.cnt) ? 0.f : 1.f / L;
-          uint16_t* out = p.o.row(pc.b, h * p.group + n - tok * p.group, tok) + 16 * kMT * warp + 2 * g;
+          const int tok = token_of(p, n);
+          const float inv = (l[nt][e] == 0.f || tok >= s.cnt) ? 0.f : 1.f / l[nt][e];
+          uint16_t* out = p.o.row(s.b, h * p.group + n - tok * p.group, tok) + 2 * g;
 #pragma unroll
-          for (int c = 0; c < kMT; ++c) {
-            const uint32_t v = inv == 0.f ? 0u : Elem<kBf16>::pack(acc[nt][c][e] * inv, acc[nt][c][2 + e] * inv);
-            *reinterpret_cast<uint32_t*>(out + 16 * c) = v;
-          }
+          for (int c = 0; c < kChunks; ++c)
+            *reinterpret_cast<uint32_t*>(out + 16 * c) =
+                inv == 0.f ? 0u : Elem<kBf16>::pack(acc[nt][c][e] * inv, acc[nt][c][2 + e] * inv);
         }
-      sync_consumers();  // sm.mx is written again by the next piece
       continue;
     }
-    // ---- a part of a unit: leave it for the CTA that finishes last
-    constexpr int kPieceFloats = kRows * (2 + kD);
-    const int c0 = owner(pc.unit_begin, total, n_split), c1 = owner(pc.unit_begin + s.items - 1, total, n_split);
-    auto piece_of = [&](int cta) {  // a CTA's first piece is its slot 0, a later one (a unit's begin) slot 1
-      const int slot = cta == c0 && split_at(c0, total, n_split) != pc.unit_begin ? 1 : 0;
-      return p.partials + (int64_t(cta) * 2 + slot) * kPieceFloats;
-    };
-    {
-      float* out = piece_of(blockIdx.x);
+    // a part of a unit: left for the CTA's end
+    // (in its stages where one warp has done its last step)
+    float* data = kR == 1 && k == n_steps - 1 ? reinterpret_cast<float*>(sm.stage[w])
+                                              : p.partials + (int64_t(worker) * 2 + (begins ? 1 : 0)) * kPiece;
+    if (wr == 0 && lane == 0)
+      sm.part[w][begins ? 1 : 0] = Part{static_cast<int>(x0) + k - s.step, data, s.b, s.sub, s.cnt, s.steps,
+                                        kFirst | (begins ? kBegin : 0) | (s.flags & kEnd)};
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+    for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = 8 * nt + 2 * t + e;
-          if (warp == 0 && g == 0) __stcg(reinterpret_cast<float2*>(out) + r, make_float2(m[nt][e], e ? sum[nt].y : sum[nt].x));
-          float* o = out + 2 * kRows + r * kD + 16 * kMT * warp + 2 * g;
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * kNT * wr + 8 * nt + 2 * t + e;
+        if (g == 0) reinterpret_cast<float2*>(data)[r] = make_float2(m[nt][e], l[nt][e]);
+        float* o = data + 2 * kRows + r * kD + 2 * g;
 #pragma unroll
-          for (int c = 0; c < kMT; ++c)
-            __stcg(reinterpret_cast<float2*>(o + 16 * c), make_float2(acc[nt][c][e], acc[nt][c][2 + e]));
-        }
-    }
-    __threadfence();
-    sync_consumers();
-    if (tid == 0) sm.ticket = atomicAdd(p.tickets + c0, 1);
-    sync_consumers();
-    if (sm.ticket != c1 - c0) continue;
-    __threadfence();
-    if (tid == 0) p.tickets[c0] = 0;  // ready for the next launch
-    // a warp takes every fourth row, a lane kD / 32 of its columns
-    constexpr int kCols = kD / 32;
-    for (int r = warp; r < kRows && n0 + r < p.rows; r += kWarps) {
-      float M = -INFINITY;
-      for (int i = c0 + lane; i <= c1; i += 32) M = fmaxf(M, __ldcg(reinterpret_cast<const float2*>(piece_of(i)) + r).x);
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-      const float ref = M == -INFINITY ? 0.f : M;
-      float L = 0.f, a[kCols];
-#pragma unroll
-      for (int j = 0; j < kCols; ++j) a[j] = 0.f;
-      for (int i0 = c0; i0 <= c1; i0 += 32) {
-        float w = 0.f, part = 0.f;
-        if (i0 + lane <= c1) {
-          const float2 ml = __ldcg(reinterpret_cast<const float2*>(piece_of(i0 + lane)) + r);
-          w = fast_exp2(ml.x - ref);
-          part = ml.x == -INFINITY ? ml.y : w * ml.y;  // (a row of NaN has no maximum; its sum is NaN)
-        }
-        L += part;
-        const int cnt = min(32, c1 - i0 + 1);
-#pragma unroll 4
-        for (int j = 0; j < cnt; ++j) {
-          const float wj = __shfl_sync(0xffffffffu, w, j);
-          const float* src = piece_of(i0 + j) + 2 * kRows + r * kD + lane * kCols;
-          float v[kCols];
-          if constexpr (kCols == 4) {
-            const float4 x = __ldcg(reinterpret_cast<const float4*>(src));
-            v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w;
-          } else {
-            const float2 x = __ldcg(reinterpret_cast<const float2*>(src));
-            v[0] = x.x, v[1] = x.y;
-          }
-#pragma unroll
-          for (int k = 0; k < kCols; ++k) a[k] += wj * v[k];
-        }
+        for (int c = 0; c < kChunks; ++c)
+          *reinterpret_cast<float2*>(o + 16 * c) = make_float2(acc[nt][c][e], acc[nt][c][2 + e]);
       }
+  }
+
+  // ---- cut units.  The CTA's parts in order (entry 2w + slot: slot 0 goes on
+  // from the worker before, slot 1 begins a unit) form runs, one per unit.
+  __syncthreads();
+  const int e_flags = lane < 2 * kWorkers ? sm.part[lane >> 1][lane & 1].flags : 0;
+  const uint32_t valid = __ballot_sync(0xffffffffu, e_flags != 0);
+  if (valid == 0) return;
+  const uint32_t begin_mask = __ballot_sync(0xffffffffu, e_flags & kBegin), end_mask = __ballot_sync(0xffffffffu, e_flags & kEnd);
+  const uint32_t run_starts = begin_mask | (valid & -valid);
+  constexpr int kCols = kD / 32;
+  auto store_row = [&](const Part& u, int row, float L, const float (&a)[kCols]) {
+    const int h = head_of(u.sub), n = (u.sub - h * p.row_tiles) * kRows + row;
+    if (n >= p.rows) return;
+    const int tok = token_of(p, n);
+    const float inv = (L == 0.f || tok >= u.cnt) ? 0.f : 1.f / L;
+    uint16_t* out = p.o.row(u.b, h * p.group + n - tok * p.group, tok) + lane * kCols;
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
-      const int n = n0 + r, tok = n / p.group;
-      const float inv = (L == 0.f || tok >= s.cnt) ? 0.f : 1.f / L;
-      uint16_t* out = p.o.row(pc.b, h * p.group + n - tok * p.group, tok) + lane * kCols;
+    for (int k = 0; k < kCols; k += 2)
+      *reinterpret_cast<uint32_t*>(out + k) = inv == 0.f ? 0u : Elem<kBf16>::pack(a[k] * inv, a[k + 1] * inv);
+  };
+  float* const cta_parts = p.partials + int64_t(gridDim.x) * kWorkers * 2 * kPiece;
+  int cut[2] = {-1, -1};  // first entries of the runs that other CTAs share: going on from one, and begun here
+  int task = 0;
+  for (uint32_t left = run_starts; left; left &= left - 1) {
+    const int first = __ffs(left) - 1;
+    const uint32_t later = left & (left - 1);
+    const uint32_t in_run = valid & ~((1u << first) - 1u) & (later ? (later & -later) - 1u : 0xffffffffu);
+    const int last = 31 - __clz(in_run), n = __popc(in_run);
+    const bool b = (begin_mask >> first) & 1, whole = b && ((end_mask >> last) & 1);
+    if (!whole) cut[b] = first;
+    const Part u = sm.part[first >> 1][first & 1];
+    for (int row = 0; row < kRows; ++row, ++task) {
+      if (task % H::kWarps != warp) continue;
+      float M, L, a[kCols];
+      // entries of a run: its first, then slot 0 of the workers behind
+      merge_row<kD, kRows, false>(n, row, lane, [&](int i) {
+        return const_cast<const float*>(i == 0 ? sm.part[first >> 1][first & 1].data : sm.part[(first >> 1) + i][0].data);
+      }, M, L, a);
+      if (whole) {
+        store_row(u, row, L, a);
+      } else {
+        float* data = cta_parts + (int64_t(blockIdx.x) * 2 + b) * kPiece;
+        if (lane == 0) __stcg(reinterpret_cast<float2*>(data) + row, make_float2(M, L));
+        float* o = data + 2 * kRows + row * kD + lane * kCols;
 #pragma unroll
-      for (int k = 0; k < kCols; k += 2)
-        *reinterpret_cast<uint32_t*>(out + k) = inv == 0.f ? 0u : Elem<kBf16>::pack(a[k] * inv, a[k + 1] * inv);
+        for (int k = 0; k < kCols; k += 2) __stcg(reinterpret_cast<float2*>(o + k), make_float2(a[k], a[k + 1]));
+      }
+    }
+  }
+  if (cut[0] < 0 && cut[1] < 0) return;
+  __threadfence();
+  __syncthreads();
+  auto cta_of = [&](int x) { return static_cast<int>(split.owner(x) / kWorkers); };
+  if (tid < 2) {
+    sm.last[tid] = 0;
+    const int c = tid ? cut[1] : cut[0];
+    if (c >= 0) {
+      const Part& u = sm.part[c >> 1][c & 1];
+      const int c0 = cta_of(u.unit_begin), c1 = cta_of(u.unit_begin + u.steps - 1);
+      sm.last[tid] = atomicAdd(p.tickets + c0, 1) == c1 - c0;
+      if (sm.last[tid]) p.tickets[c0] = 0;  // ready for the next launch
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int side = 0; side < 2; ++side) {
+    if (!sm.last[side]) continue;
+    __threadfence();
+    const Part u = sm.part[cut[side] >> 1][cut[side] & 1];
+    const int c0 = cta_of(u.unit_begin), c1 = cta_of(u.unit_begin + u.steps - 1);
+    // the first CTA's part begins there, the others' go on from the one before
+    for (int row = warp; row < kRows; row += H::kWarps) {
+      float M, L, a[kCols];
+      merge_row<kD, kRows, true>(c1 - c0 + 1, row, lane, [&](int i) {
+        return const_cast<const float*>(cta_parts + (int64_t(c0 + i) * 2 + (i == 0)) * kPiece);
+      }, M, L, a);
+      store_row(u, row, L, a);
     }
   }
 }
 
 struct Plan {
-  int nt, row_tiles, n_ctas;
+  int nt, r, row_tiles, workers, n_ctas;
   size_t bytes;
 };
 
 int max_ctas() {
   const int sms = current_device().sm_count;
-  return kCtasPerSm * (sms > 0 ? sms : 148);
+  return sms > 0 ? sms : 148;
 }
 
-// Query rows of a KV head: up to 8, 16 or 32 in a unit.
+// Query rows of a unit: up to 8 or 16 for one warp, 32 for two, 64 for four.
 Plan plan(const nsa_kv8_cache* c, int64_t rows) {
   Plan s;
-  s.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-  s.row_tiles = static_cast<int>((rows + kRowTile - 1) / kRowTile);
-  const int64_t most = c->batch * c->n_kv_heads * s.row_tiles * c->max_blocks;  // items
-  s.n_ctas = static_cast<int>(most < max_ctas() ? most : max_ctas());
-  s.bytes = size_t(s.n_ctas) * 2 * 8 * s.nt * (2 + c->head_dim) * sizeof(float);
+  s.nt = rows <= 8 ? 1 : 2;
+  s.r = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
+  const int tile = 8 * s.nt * s.r;
+  s.row_tiles = static_cast<int>((rows + tile - 1) / tile);
+  s.workers = (s.nt == 1 ? 12 : 8) / s.r;
+  const int64_t most = c->batch * c->n_kv_heads * s.row_tiles * (2 * c->max_blocks + 4);  // steps
+  const int64_t ctas = (most + s.workers - 1) / s.workers;
+  s.n_ctas = static_cast<int>(ctas < max_ctas() ? ctas : max_ctas());
+  s.bytes = size_t(s.n_ctas) * (s.workers + 1) * 2 * tile * (2 + c->head_dim) * sizeof(float);
   return s;
 }
 
-template <int kD, int kNT, bool kBf16, bool kInt8>
-int launch_attend(const CUtensorMap (&maps)[4], const AttendParams& p, cudaStream_t stream) {
-  using S = Smem<kD, kNT>;
-  static_assert(offsetof(S, stage) == 0 && Geo<kD>::kStageBytes % 1024 == 0, "TMA destinations");
-  static_assert(offsetof(S, q) % 16 == 0 && Geo<kD>::kQStride % 16 == 0, "bulk-copy destinations");
-  static_assert(offsetof(S, p_hi) % 16 == 0 && offsetof(S, p_lo) % 16 == 0 && offsetof(S, mx) % 8 == 0, "vector reads");
-  static_assert(kCtasPerSm * (sizeof(S) + 1024) <= 228 * 1024, "two CTAs per SM");
-  auto kernel = kv8_attend_kernel<kD, kNT, kBf16, kInt8>;
+template <int kD, int kNT, int kR, bool kBf16, bool kInt8>
+int launch_attend(const Plan& plan, const CUtensorMap (&maps)[4], const AttendParams& p, cudaStream_t stream) {
+  using S = Smem<kNT, kR>;
+  using H = Shape<kNT, kR>;
+  static_assert(offsetof(S, stage) == 0 && offsetof(S, step) % 16 == 0, "TMA destinations, vector reads");
+  static_assert(sizeof(S) <= 227 * 1024, "shared memory of an SM");
+  static_assert(2 * H::kWorkers <= 32, "a lane for each part");
+  auto kernel = kv8_attend_kernel<kD, kNT, kR, kBf16, kInt8>;
   static bool attr_set[64] = {false};
   const int dev = current_device().device;
   if (dev < 0 || dev >= 64) return fail(NSA_ERR_CUDA, "no CUDA device");
@@ -1008,19 +951,18 @@ int launch_attend(const CUtensorMap (&maps)[4], const AttendParams& p, cudaStrea
     if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
     attr_set[dev] = true;
   }
-  cudaError_t e = launch_kernel(kernel, dim3(p.n_ctas), dim3(kThreads), sizeof(S), stream, maps[0], maps[1], maps[2],
-                                maps[3], p);
+  cudaError_t e = launch_kernel(kernel, dim3(plan.n_ctas), dim3(H::kThreads), sizeof(S), stream, maps[0], maps[1],
+                                maps[2], maps[3], p);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? NSA_OK : cuda_fail(e, "kv8_attend_kernel launch");
 }
 
 template <int kD, bool kBf16, bool kInt8>
-int launch_nt(int nt, const CUtensorMap (&maps)[4], const AttendParams& p, cudaStream_t stream) {
-  switch (nt) {
-    case 1: return launch_attend<kD, 1, kBf16, kInt8>(maps, p, stream);
-    case 2: return launch_attend<kD, 2, kBf16, kInt8>(maps, p, stream);
-    default: return launch_attend<kD, 4, kBf16, kInt8>(maps, p, stream);
-  }
+int launch_rows(const Plan& s, const CUtensorMap (&maps)[4], const AttendParams& p, cudaStream_t stream) {
+  if (s.nt == 1) return launch_attend<kD, 1, 1, kBf16, kInt8>(s, maps, p, stream);
+  if (s.r == 1) return launch_attend<kD, 2, 1, kBf16, kInt8>(s, maps, p, stream);
+  if (s.r == 2) return launch_attend<kD, 2, 2, kBf16, kInt8>(s, maps, p, stream);
+  return launch_attend<kD, 2, 4, kBf16, kInt8>(s, maps, p, stream);
 }
 
 int check_shape(const nsa_kv8_cache* cache, int64_t n_heads, int64_t n_tokens) {
@@ -1067,6 +1009,8 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
   p.n_tokens = static_cast<int>(n_tokens);
   p.rows = p.group * p.n_tokens;
   const kv8::Plan s = kv8::plan(cache, p.rows);
+  if (int64_t(p.c.n_kv_heads) * s.row_tiles * (2 * int64_t(p.c.max_blocks) + 4) > 0x7fffffff)
+    return fail(NSA_ERR_UNSUPPORTED, "too many (head, block) pairs in a sequence");
   if (!workspace || workspace_bytes < s.bytes)
     return fail(NSA_ERR_WORKSPACE, "workspace of %zu bytes required (got %zu)", s.bytes, workspace ? workspace_bytes : size_t(0));
   if (!aligned16(workspace)) return fail(NSA_ERR_ALIGN, "workspace must be 16-byte aligned");
@@ -1076,7 +1020,7 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
   p.window = window < 0 ? -1 : static_cast<int>(window);
   p.sink = static_cast<int>(sink);
   p.scale_log2 = sm_scale * kv8::kLog2e;
-  p.n_ctas = s.n_ctas;
+  p.group_inv = p.group > 1 ? static_cast<uint32_t>(((uint64_t(1) << 32) + p.group - 1) / p.group) : 0;
   p.tickets = tickets;
   p.partials = static_cast<float*>(workspace);
   p.err = device_error_word();
@@ -1086,7 +1030,7 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
   const uint64_t code_dims[2] = {d, static_cast<uint64_t>(p.c.n_pages) * p.c.n_kv_heads * kv8::kBlock};
   const uint64_t ring_dims[2] = {d, static_cast<uint64_t>(p.c.batch) * p.c.n_kv_heads * kv8::kRing};
   const uint64_t code_stride[1] = {d}, ring_stride[1] = {2 * d};
-  const uint32_t code_box[2] = {static_cast<uint32_t>(d), kv8::kBlock}, ring_box[2] = {64, 8};
+  const uint32_t code_box[2] = {static_cast<uint32_t>(d), static_cast<uint32_t>(4096 / d)}, ring_box[2] = {64, 8};
   const CUtensorMapSwizzle swz = d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap maps[4];
   const void* base[4] = {p.c.k_codes, p.c.v_codes, p.c.k_ring, p.c.v_ring};
@@ -1098,14 +1042,14 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
   }
   const bool bf16 = cache->dtype == 2, int8 = cache->codes == NSA_KV8_INT8;
   if (d == 128)
-    return bf16 ? (int8 ? kv8::launch_nt<128, true, true>(s.nt, maps, p, stream)
-                        : kv8::launch_nt<128, true, false>(s.nt, maps, p, stream))
-                : (int8 ? kv8::launch_nt<128, false, true>(s.nt, maps, p, stream)
-                        : kv8::launch_nt<128, false, false>(s.nt, maps, p, stream));
-  return bf16 ? (int8 ? kv8::launch_nt<64, true, true>(s.nt, maps, p, stream)
-                      : kv8::launch_nt<64, true, false>(s.nt, maps, p, stream))
-              : (int8 ? kv8::launch_nt<64, false, true>(s.nt, maps, p, stream)
-                      : kv8::launch_nt<64, false, false>(s.nt, maps, p, stream));
+    return bf16 ? (int8 ? kv8::launch_rows<128, true, true>(s, maps, p, stream)
+                        : kv8::launch_rows<128, true, false>(s, maps, p, stream))
+                : (int8 ? kv8::launch_rows<128, false, true>(s, maps, p, stream)
+                        : kv8::launch_rows<128, false, false>(s, maps, p, stream));
+  return bf16 ? (int8 ? kv8::launch_rows<64, true, true>(s, maps, p, stream)
+                      : kv8::launch_rows<64, true, false>(s, maps, p, stream))
+              : (int8 ? kv8::launch_rows<64, false, true>(s, maps, p, stream)
+                      : kv8::launch_rows<64, false, false>(s, maps, p, stream));
 }
 
 int nsa_kv8_decode_step(const nsa_kv8_cache* cache, const nsa_kv8_rows* new_k, const nsa_kv8_rows* new_v,

@@ -16,6 +16,7 @@ number of query heads per KV head, ragged batches and several query tokens.
 from __future__ import annotations
 
 import ctypes
+import threading
 
 import torch
 
@@ -28,7 +29,39 @@ MAX_QUERY = 64  # query tokens of one attend
 
 _CODES = {"e4m3": (0, torch.float8_e4m3fn), "int8": (1, torch.int8)}
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_GRAPH_SLOTS = 256
+
+# Scratch of attention.  Eager calls share one (workspace, tickets) pair per
+# (device, stream).  A call captured into a graph takes its workspace from the
+# graph's own pool and one of _GRAPH_ROWS ticket rows (in turn), so that graphs
+# replayed side by side do not share them.
+_GRAPH_ROWS = 4096
+_scratch_lock = threading.Lock()
+_eager: dict = {}
+_graph: dict = {}  # device index -> [rows, next]
+
+
+def _graph_rows(device):
+    """Ticket rows for captured calls, made before any capture (when a cache is)."""
+    with _scratch_lock:
+        if device.index not in _graph:
+            with _lib.on_device(device):
+                n = int(_lib.load().nsa_kv8_ticket_count())
+            _graph[device.index] = [torch.zeros((_GRAPH_ROWS, n), dtype=torch.int32, device=device), 0]
+
+
+def _scratch(device, nbytes, stream):
+    if torch.cuda.is_current_stream_capturing():
+        with _scratch_lock:
+            slot = _graph[device.index]
+            row = slot[1]
+            slot[1] = (row + 1) % _GRAPH_ROWS
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), slot[0][row]
+    pair = _eager.get((device.index, stream))
+    if pair is None or pair[0].numel() < nbytes:
+        with _scratch_lock:
+            tickets = pair[1] if pair else torch.zeros_like(_graph[device.index][0][0])
+            pair = _eager[(device.index, stream)] = (torch.empty(nbytes, dtype=torch.uint8, device=device), tickets)
+    return pair
 
 
 def _req(cond, msg, exc=ValueError):
@@ -112,12 +145,8 @@ class Kv8Cache:
                      ("lens", self.lens), ("ring_floor", self._ring_floor), ("tickets", self._append_tickets)):
             setattr(d, n, t.data_ptr())
         self._desc_ref = ctypes.byref(d)
-        lib = _lib.load()
-        with _lib.on_device(device):
-            self._n_tickets = int(lib.nsa_kv8_ticket_count())
-        self._graph_tickets = z((_GRAPH_SLOTS, self._n_tickets), torch.int32)
-        self._graph_calls = 0
-        self._ws_bytes, self._eager = {}, {}
+        self._ws_bytes = {}
+        _graph_rows(device)
 
     # ---------------------------------------------------------------- plumbing
     def _check(self, name, t, heads):
@@ -143,26 +172,14 @@ class Kv8Cache:
         return t.data_ptr()
 
     def _scratch(self, heads, n_tokens, stream):
-        """Workspace and tickets of one attend.  Eager calls: one pair per
-        stream.  A call captured into a graph: workspace from the graph's own
-        pool and a ticket row of its own (256 rows, then from the start again),
-        so that graphs replayed side by side do not share them."""
-        key = (heads, n_tokens)
-        nbytes = self._ws_bytes.get(key)
+        """Workspace and tickets of one attend."""
+        nbytes = self._ws_bytes.get((heads, n_tokens))
         if nbytes is None:
             nbytes = _lib.load().nsa_kv8_workspace_bytes(self._desc_ref, heads, n_tokens)
             if self.batch and not nbytes:
                 _lib.check(_lib.NSA_ERR_INVALID)  # raises with the library's message
-            self._ws_bytes[key] = nbytes
-        if torch.cuda.is_current_stream_capturing():
-            tickets = self._graph_tickets[self._graph_calls % _GRAPH_SLOTS]
-            self._graph_calls += 1
-            return torch.empty(nbytes, dtype=torch.uint8, device=self.device), tickets
-        pair = self._eager.get(stream)
-        if pair is None or pair[0].numel() < nbytes:
-            tickets = pair[1] if pair else torch.zeros(self._n_tickets, dtype=torch.int32, device=self.device)
-            pair = self._eager[stream] = (torch.empty(nbytes, dtype=torch.uint8, device=self.device), tickets)
-        return pair
+            self._ws_bytes[heads, n_tokens] = nbytes
+        return _scratch(self.device, nbytes, stream)
 
     def _mask(self, window, sink):
         window, sink = -1 if window is None else int(window), int(sink)
