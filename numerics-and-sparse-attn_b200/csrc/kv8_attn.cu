@@ -15,16 +15,15 @@
 // of 64 or 128 rows; here the conversion happens in registers on the way from
 // ldmatrix to the mma.
 //
-// Work is split evenly over independent workers by steps: a step is 32 or 64
-// tokens of a block (8 KiB of codes), or 16 or 32 tokens of a sequence's
-// incomplete block in the ring.  The lengths live on the device, so every CTA
-// computes the split itself (one scan over the batch).  A worker is one warp
-// (up to 16 query rows) or 2 or 4 warps (32, 64 rows) that share its copies; it
-// issues its own TMA loads, two or more steps ahead, and keeps scores, P and
-// accumulators in registers, so no warp waits for another until its steps are
-// done.  A worker's consecutive steps form pieces of units (sequence, KV head,
-// row tile).  Units cut between workers are merged by the CTA at its end, and
-// those cut between CTAs by the last of them to finish.
+// Work is split evenly over independent workers (warps) by steps: a step is a
+// block of 64 tokens, or 32 tokens of a sequence's incomplete block in the
+// ring.  The lengths live on the device, so every CTA computes the split itself
+// (one scan over the batch).  A worker issues its own TMA loads -- the next K as
+// soon as the scores are done, the next V as soon as the sums are -- and keeps
+// scores, P and accumulators in registers, so no warp waits for another until
+// its steps are done.  A worker's consecutive steps form pieces of units
+// (sequence, KV head, row tile).  Units cut between workers are merged by the
+// CTA at its end, and those cut between CTAs by the last of them to finish.
 #include <cstddef>
 #include <cstdlib>
 
@@ -34,9 +33,7 @@ namespace nsa {
 namespace kv8 {
 namespace {
 
-constexpr uint32_t kHalf = 4096;     // bytes of K, and of V, in a stage
-constexpr uint32_t kStageBytes = 2 * kHalf;
-constexpr int kLensCached = 1024;    // sequence lengths kept in shared memory
+constexpr int kLensCached = 512;  // sequence lengths kept in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct AttendParams {
@@ -48,7 +45,7 @@ struct AttendParams {
   int window, sink;  // window < 0: all positions
   float scale_log2;
   int* tickets;     // [CTAs]
-  float* partials;  // [workers][2] pieces, then [CTAs][2]: m and l of every row, then kD sums a row
+  float* partials;  // [workers][2] pieces, then [CTAs][2]: maximum and sum of every row, then kD sums a row
   int* err;
 };
 
@@ -58,12 +55,12 @@ __device__ __forceinline__ int token_of(const AttendParams& p, int n) {
   return p.group == 1 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), p.group_inv));
 }
 
+constexpr int kRingTok = 32;  // tokens of a ring step
+
 template <int kD>
 struct Geo {
-  static constexpr int kTok = kHalf / kD;          // tokens of a block step
-  static constexpr int kSteps = kBlock / kTok;     // steps of a block
-  static constexpr int kRingTok = kHalf / (2 * kD);  // tokens of a ring step
-  static constexpr uint32_t kRegions = kD / 64;    // 128-byte column parts of a ring step
+  static constexpr uint32_t kHalf = kBlock * kD;  // bytes of K, and of V, of a step (ring: 32 tokens of 2 bytes)
+  static constexpr uint32_t kRegions = kD / 64;   // 128-byte column parts of a ring step
   static constexpr uint32_t kRegion = kRingTok * 128;
 };
 
@@ -76,9 +73,7 @@ struct Seq {
   bool empty;                  // nothing to see: its one step writes zeros
 };
 
-template <int kD>
 __device__ __forceinline__ Seq make_seq(const AttendParams& p, int len, int cnt) {
-  using G = Geo<kD>;
   Seq s;
   s.len = len;
   s.cnt = cnt;
@@ -89,7 +84,7 @@ __device__ __forceinline__ Seq make_seq(const AttendParams& p, int len, int cnt)
     s.sink_blocks = min((p.sink + kBlock - 1) / kBlock, s.full);
     s.win_block = min(max(max(len - cnt + 1 - p.window, 0) / kBlock, s.sink_blocks), s.full);
   }
-  s.steps = (s.sink_blocks + s.full - s.win_block) * G::kSteps + (len % kBlock + G::kRingTok - 1) / G::kRingTok;
+  s.steps = s.sink_blocks + s.full - s.win_block + (len % kBlock + kRingTok - 1) / kRingTok;
   s.empty = cnt == 0 || s.steps == 0;
   if (s.empty) s.steps = 1;
   return s;
@@ -135,28 +130,32 @@ struct Part {
   int flags;  // 0: none; else kFirst and whether it holds the unit's begin / end
 };
 
-// Warps of a CTA (one per SM), warps of a worker, stages of a worker: 24 stages
-// of 8 KiB in flight an SM.
-template <int kNT, int kR>
+// One CTA per SM.  12 warps of 168 registers where 8 query rows leave room for
+// them, else 8 of 255; the shared memory left over goes to their stages.  With 32
+// rows the query fragments are read from shared memory (64 registers of 128
+// dimensions otherwise).
+template <int kD, int kNT, bool kSplit>
 struct Shape {
   static constexpr int kWarps = kNT == 1 ? 12 : 8;
-  static constexpr int kWorkers = kWarps / kR;
-  static constexpr int kStages = 24 / kWorkers;
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kRows = 8 * kNT * kR;  // of a unit
+  static constexpr int kRows = 8 * kNT;  // of a unit
+  static constexpr bool kQShared = kNT == 4;
+  static constexpr int kQStride = kD * 2 + 32;  // bytes: rows 8 banks apart
+  static constexpr int kTok = kNT == 4 ? 16 : kNT == 2 || kSplit ? 32 : 64;  // tokens of a round of scores, softmax and sums
 };
 
-template <int kNT, int kR>
+template <int kD, int kNT, bool kSplit>
 struct Smem {
-  using H = Shape<kNT, kR>;
-  uint8_t stage[H::kWorkers][H::kStages][kStageBytes];  // 1024-aligned: TMA destinations
-  Step step[H::kWorkers][H::kStages];
-  Part part[H::kWorkers][2];
+  using H = Shape<kD, kNT, kSplit>;
+  uint8_t stage[H::kWarps][2 * Geo<kD>::kHalf];  // K, V; 1024-aligned: TMA destinations
+  uint8_t q[H::kWarps][H::kRows][H::kQStride];
+  Step step[H::kWarps][2];
+  Part part[H::kWarps][2];
   int2 lens[kLensCached];
   int scan[H::kWarps];
   int before[H::kThreads];  // steps before a thread's sequences
   int last[2];  // whether this CTA was the last of its first / last cut unit
-  uint64_t full[H::kWorkers][H::kStages], empty[H::kWorkers][H::kStages];
+  uint64_t k_full[H::kWarps], v_full[H::kWarps];
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -176,38 +175,48 @@ __device__ __forceinline__ void mma_elem(float (&d)[4], uint32_t a0, uint32_t a1
     mma_16816(d, a0, a1, a2, a3, b0, b1);
 }
 
-// Four codes to two fp16 pairs: (bytes 0, 1) and (2, 3), or with kSplit
-// (0, 2) and (1, 3).  int8: the byte, biased by 128, is the low part of an
+// D = A * B (mma_16816 without a sum to go on from).
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Two 16 x 16 matrices of bytes, transposed: lane (g, t) gets of each the rows
+// 4t .. 4t + 3 of columns g and g + 8.
+__device__ __forceinline__ void ldmatrix_b8_trans(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
+                                                  uint32_t& r3) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
+               : "r"(addr));
+}
+
+// Four codes to two fp16 pairs.  int8: the byte, biased by 128, is the low part of an
 // fp16 number in [1024, 2048), from which 1152 is taken again (exact).
-template <bool kInt8, bool kSplit>
+template <bool kInt8>
 __device__ __forceinline__ void to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if constexpr (kInt8) {
     const uint32_t x = w ^ 0x80808080u, magic = 0x64646464u;
-    const uint32_t a = __byte_perm(x, magic, kSplit ? 0x4240 : 0x4140);
-    const uint32_t b = __byte_perm(x, magic, kSplit ? 0x4341 : 0x4342);
+    const uint32_t a = __byte_perm(x, magic, 0x4140);
+    const uint32_t b = __byte_perm(x, magic, 0x4342);
     const __half2 bias = __float2half2_rn(1152.f);
     const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&a), bias);
     const __half2 z = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
     lo = *reinterpret_cast<const uint32_t*>(&y);
     hi = *reinterpret_cast<const uint32_t*>(&z);
   } else {
-    const uint32_t x = kSplit ? __byte_perm(w, 0u, 0x3120) : w;
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
         "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
         : "=r"(lo), "=r"(hi)
-        : "r"(x));
+        : "r"(w));
   }
 }
 
 __device__ __forceinline__ void lds8(uint32_t addr, uint32_t& lo, uint32_t& hi) {
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo), "=r"(hi) : "r"(addr));
 }
-__device__ __forceinline__ uint32_t lds4(uint32_t addr) {
-  uint32_t x;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(x) : "r"(addr));
-  return x;
-}
-
 // A pair of fp16 numbers of 8 significant bits as bf16 (exact).  volatile, so
 // that the conversions of all query fragments stay on the ring's path instead
 // of being kept in registers.
@@ -295,23 +304,24 @@ __device__ __forceinline__ void merge_row(int n, int row, int lane, Ptr ptr, flo
   for (int off = 16; off > 0; off >>= 1) L += __shfl_xor_sync(0xffffffffu, L, off);
 }
 
-template <int kD, int kNT, int kR, bool kBf16, bool kInt8>
-__global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
+template <int kD, int kNT, bool kBf16, bool kInt8>
+__global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
     kv8_attend_kernel(const __grid_constant__ CUtensorMap tm_kc, const __grid_constant__ CUtensorMap tm_vc,
                       const __grid_constant__ CUtensorMap tm_kr, const __grid_constant__ CUtensorMap tm_vr,
                       const AttendParams p) {
   using G = Geo<kD>;
-  using H = Shape<kNT, kR>;
-  using S = Smem<kNT, kR>;
-  constexpr int kWorkers = H::kWorkers, kStages = H::kStages, kRows = H::kRows;
-  constexpr int kChunks = kD / 16;         // 16-wide steps of the head dimension
-  constexpr int kTC = G::kTok / 16;        // 16-token steps of a block step
-  constexpr int kRC = G::kRingTok / 16;    // and of a ring step
-  constexpr int kPiece = kRows * (2 + kD);  // floats of a partial result
   // P as one fp16 number has a relative error of 2^-12, the same as rounding
   // the output to fp16 makes, and far below bf16's.  With fp16 outputs P is
   // the sum of two fp16 numbers (2^-23).
   constexpr bool kSplitP = !kBf16;
+  using H = Shape<kD, kNT, kSplitP>;
+  using S = Smem<kD, kNT, kSplitP>;
+  constexpr int kRows = H::kRows;
+  constexpr int kChunks = kD / 16;              // 16-wide steps of the head dimension
+  constexpr int kTC = H::kTok / 16;             // 16-token parts of a round
+  constexpr int kRounds = kBlock / H::kTok;
+  constexpr int kRC = kTC < kRingTok / 16 ? kTC : kRingTok / 16;  // of a round of a ring step
+  constexpr int kPiece = kRows * (2 + kD);      // floats of a partial result
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   grid_launch_dependents();
   if (smem_u32(smem_raw) & 1023u) {
@@ -320,13 +330,12 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
   }
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const int w = warp / kR, wr = warp % kR;  // worker; its warp
-  if (tid < kWorkers * kStages) {
-    mbar_init(smem_u32(&sm.full[0][0] + tid), 1);
-    mbar_init(smem_u32(&sm.empty[0][0] + tid), kR);
+  if (tid < H::kWarps) {
+    mbar_init(smem_u32(&sm.k_full[tid]), 1);
+    mbar_init(smem_u32(&sm.v_full[tid]), 1);
     fence_barrier_init();
   }
-  if (tid < 2 * kWorkers) sm.part[tid >> 1][tid & 1].flags = 0;
+  if (tid < 2 * H::kWarps) sm.part[tid >> 1][tid & 1].flags = 0;
   if (tid == H::kThreads - 1) {
     prefetch_tmap(&tm_kc);
     prefetch_tmap(&tm_vc);
@@ -342,7 +351,7 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
   for (int b = tid * per; b < min(batch, (tid + 1) * per); ++b) {
     const int2 l = load_len(p, b);
     if (b < kLensCached) sm.lens[b] = l;
-    mine += make_seq<kD>(p, l.x, l.y).steps;
+    mine += make_seq(p, l.x, l.y).steps;
   }
   int before = mine;
 #pragma unroll
@@ -362,21 +371,20 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
     if (tid == 0) set_error(p.err, NSA_ERR_INVALID);
     return;
   }
-  const Split split(static_cast<uint32_t>(sum) * units, gridDim.x * kWorkers);
-  if (blockIdx.x * kWorkers >= split.n) return;  // the whole CTA has nothing to do
-  const uint32_t worker = blockIdx.x * kWorkers + w;
+  const Split split(static_cast<uint32_t>(sum) * units, gridDim.x * H::kWarps);
+  if (blockIdx.x * H::kWarps >= split.n) return;  // the whole CTA has nothing to do
+  const uint32_t worker = blockIdx.x * H::kWarps + warp;
   const uint32_t x0 = worker < split.n ? split.begin(worker) : split.total;
   const int n_steps = worker < split.n ? static_cast<int>(split.begin(worker + 1) - x0) : 0;
   sm.before[tid] = before + prior - mine;
   __syncthreads();
 
-  // ---- issuing (a worker's first warp): lane i knows step batch0 + i
-  int cur_b = 0, batch0 = -32, issued = 0;
+  // ---- issuing: lane i knows step batch0 + i
+  int cur_b = 0, batch0 = -32;
   int cur_rel = 0;  // first step of sequence cur_b, from the worker's first
-  uint32_t i_st = 0, i_ph = 0;
   Step mystep{};
   int myrow = 0;
-  if (wr == 0 && n_steps > 0) {  // the sequence of the first step: the last one that begins at it or before
+  if (n_steps > 0) {  // the sequence of the first step: the last one that begins at it or before
     const int at = static_cast<int>(x0 / units), threads = (batch + per - 1) / per;
     int n = 0;
     for (int i = lane; i < threads; i += 32) n += sm.before[i] <= at;
@@ -385,7 +393,7 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
     int begin = sm.before[n];
     for (;;) {
       const int2 l = cur_b < kLensCached ? sm.lens[cur_b] : load_len(p, cur_b);
-      const int steps = make_seq<kD>(p, l.x, l.y).steps;
+      const int steps = make_seq(p, l.x, l.y).steps;
       if (at < begin + steps) break;
       begin += steps;
       ++cur_b;
@@ -404,7 +412,7 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
     int step = 0, sub = 0, b = 0;
     for (;;) {
       const int2 l = cur_b < kLensCached ? sm.lens[cur_b] : load_len(p, cur_b);
-      const Seq c = make_seq<kD>(p, l.x, l.y);
+      const Seq c = make_seq(p, l.x, l.y);
       const int end = cur_rel + c.steps * units;
       if (!found && k < end) {
         const uint32_t off = static_cast<uint32_t>(k - cur_rel);
@@ -430,12 +438,11 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
     mystep.ks = mystep.vs = 1.f;
     int flags = (step == 0 ? kBegin | kFirst : 0) | (step == s.steps - 1 ? kEnd | kLast : 0);
     flags |= (k == 0 ? kFirst : 0) | (k == n_steps - 1 ? kLast : 0);
-    const int block_steps = (s.sink_blocks + s.full - s.win_block) * G::kSteps;
+    const int blocks = s.sink_blocks + s.full - s.win_block;
     if (s.empty) {
       flags |= kEmpty;
-    } else if (step < block_steps) {
-      const int item = step / G::kSteps, tok = (step % G::kSteps) * G::kTok;
-      const int block = item < s.sink_blocks ? item : s.win_block + item - s.sink_blocks;
+    } else if (step < blocks) {
+      const int block = step < s.sink_blocks ? step : s.win_block + step - s.sink_blocks;
       int page = __ldg(p.c.page_table + int64_t(b) * p.c.max_blocks + block);
       float2 sc = make_float2(NAN, NAN);
       if (page >= 0 && page < p.c.n_pages) {
@@ -446,71 +453,85 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
       }
       mystep.ks = sc.x;
       mystep.vs = sc.y;
-      mystep.pos0 = block * kBlock + tok;
-      myrow = (page * p.c.n_kv_heads + h) * kBlock + tok;
+      mystep.pos0 = block * kBlock;
+      myrow = (page * p.c.n_kv_heads + h) * kBlock;
       const int lo = limit_at(s.len, s.cnt, n0), hi = limit_at(s.len, s.cnt, n0 + kRows - 1);
-      if (mystep.pos0 + G::kTok > lo ||
-          (p.window >= 0 && mystep.pos0 < hi - p.window && mystep.pos0 + G::kTok > p.sink))
+      if (mystep.pos0 + kBlock > lo || (p.window >= 0 && mystep.pos0 < hi - p.window && mystep.pos0 + kBlock > p.sink))
         flags |= kMasked;
     } else {
-      mystep.pos0 = s.full * kBlock + (step - block_steps) * G::kRingTok;
+      mystep.pos0 = s.full * kBlock + (step - blocks) * kRingTok;
       myrow = (b * p.c.n_kv_heads + h) * kRing + mystep.pos0 % kRing;
-      flags |= kRingStep | kMasked | (min(G::kRingTok, s.len - mystep.pos0) << 8);
+      flags |= kRingStep | kMasked | (min(kRingTok, s.len - mystep.pos0) << 8);
     }
     mystep.flags = flags;
   };
-  bool aborted = false;
-  auto issue_to = [&](int upto) {  // stages steps [issued, upto)
-    for (upto = min(upto, n_steps); issued < upto; ++issued) {
-      if (issued >= batch0 + 32) fetch(issued);
-      if (lane == issued - batch0 && !aborted) {
-        if (kR > 1 && !mbar_wait(smem_u32(&sm.empty[w][i_st]), i_ph ^ 1, p.err)) {
-          aborted = true;
-        } else {
-          const uint32_t fb = smem_u32(&sm.full[w][i_st]), dst = smem_u32(sm.stage[w][i_st]);
-          if (mystep.flags & kEmpty) {
-            sm.step[w][i_st] = mystep;
-            mbar_arrive(fb);
-          } else if (!(mystep.flags & kRingStep)) {
-            // the copies before the scales have arrived: the phase ends with the arrive below
-            tma_load_2d(dst, &tm_kc, fb, 0, myrow);
-            tma_load_2d(dst + kHalf, &tm_vc, fb, 0, myrow);
-            sm.step[w][i_st] = mystep;
-            mbar_arrive_expect_tx(fb, kStageBytes);
-          } else {
-            const int boxes = ((mystep.flags >> 8) + 7) / 8;  // of 8 slots, those that hold tokens
-            sm.step[w][i_st] = mystep;
-            mbar_arrive_expect_tx(fb, boxes * 8 * kD * 4);
-            for (int r = 0; r < boxes; ++r)
-              for (uint32_t c = 0; c < G::kRegions; ++c) {
-                tma_load_2d(dst + c * G::kRegion + r * 1024, &tm_kr, fb, c * 64, myrow + 8 * r);
-                tma_load_2d(dst + kHalf + c * G::kRegion + r * 1024, &tm_vr, fb, c * 64, myrow + 8 * r);
-              }
+  // Stages K (and with it the queries of a new piece and what is to be known of
+  // the step) or V of step k; called for k = 0, 1, ... in turn, K before V.
+  auto issue = [&](int k, bool v) {
+    if (k < n_steps) {
+      if (!v && k >= batch0 + 32) fetch(k);
+      uint32_t q_rows = 0;
+      if (!v) {
+        const int flags = __shfl_sync(0xffffffffu, mystep.flags, k - batch0);
+        if ((flags & (kFirst | kEmpty)) == kFirst) {  // a query row a lane
+          const int b = __shfl_sync(0xffffffffu, mystep.b, k - batch0), sub = __shfl_sync(0xffffffffu, mystep.sub, k - batch0);
+          const int h = head_of(sub), n0 = (sub - h * p.row_tiles) * kRows;
+          q_rows = min(kRows, p.rows - n0);
+          if (lane < q_rows) {
+            const int n = n0 + lane, tok = token_of(p, n);
+            bulk_load(smem_u32(sm.q[warp][lane]), p.q.row(b, h * p.group + n - tok * p.group, tok), kD * 2,
+                      smem_u32(&sm.k_full[warp]));
           }
         }
       }
-      if (++i_st == kStages) i_st = 0, i_ph ^= 1;
+      if (lane == k - batch0) {
+        const uint32_t fb = smem_u32(v ? &sm.v_full[warp] : &sm.k_full[warp]);
+        const uint32_t dst = smem_u32(sm.stage[warp]) + (v ? G::kHalf : 0);
+        uint32_t bytes = 0;
+        if (mystep.flags & kRingStep) {
+          const int boxes = ((mystep.flags >> 8) + 7) / 8;  // of 8 slots, those that hold tokens
+          bytes = boxes * 16 * kD;
+          for (int r = 0; r < boxes; ++r)
+            for (uint32_t c = 0; c < G::kRegions; ++c)
+              tma_load_2d(dst + c * G::kRegion + r * 1024, v ? &tm_vr : &tm_kr, fb, c * 64, myrow + 8 * r);
+        } else if (!(mystep.flags & kEmpty)) {
+          bytes = G::kHalf;
+          tma_load_2d(dst, v ? &tm_vc : &tm_kc, fb, 0, myrow);
+        }
+        // (the copies go first: the scales may still be on their way, and the phase ends with this arrival)
+        if (!v) sm.step[warp][k & 1] = mystep;
+        mbar_arrive_expect_tx(fb, bytes + q_rows * kD * 2);
+      }
     }
     __syncwarp();
   };
-  if (wr == 0) issue_to(kStages);
+  issue(0, false);
+  issue(0, true);
 
   // ---- the worker's steps.  After a wait that ran out (the error word is
   // set) a warp waits no more, so that it still reaches the CTA's barriers.
-  uint32_t qf[kNT][kChunks][2];
+  uint32_t qf[H::kQShared ? 1 : kNT][kChunks][2];
   float qscale[kNT][2];  // of rows 8nt + 2t + (0, 1): the row's power of two, sm_scale and log2(e)
   float m[kNT][2], l[kNT][2];
   int limit[kNT][2];           // positions below it are seen
-  float acc[kNT][kChunks][4];  // dims 16c + 2g (0, 1) and 16c + 2g + 1 (2, 3), rows 2t (0, 2) and 2t + 1 (1, 3)
+  float acc[kNT][kChunks][4];  // dims 16c + g (0, 1) and 16c + g + 8 (2, 3), rows 2t (0, 2) and 2t + 1 (1, 3)
   bool begins = false;         // the piece holds its unit's first step
-  uint32_t st = 0, ph = 0;
+  bool aborted = false;
+  const uint32_t q_at = smem_u32(&sm.q[warp][g][8 * t]);
+  // 16 tokens of K are rows 0..15 of a product.  Row r < 8 is token r, row 8 +
+  // j token 8 + (j ^ 4), so that the byte transposition of V, whose rows 4a +
+  // (0..3) are then rows 2a, 2a + 1, 8 + 2a and 9 + 2a of the product, reads
+  // eight different 16-byte columns of the swizzle at a time, as K does.
+  const int k_hi = (lane >> 3) & 1, k_row = 8 * k_hi + ((lane & 7) ^ (k_hi << 2));
+  const int v_a = (lane >> 2) & 3, v_j = lane & 3, v_row = v_j < 2 ? 2 * v_a + v_j : 8 + ((2 * v_a + v_j - 2) ^ 4);
+  const uint32_t k_off = k_row * kD + (((lane >> 4) ^ (kD == 128 ? (k_row & 7) : ((k_row >> 1) & 3))) << 4);
+  const uint32_t v_off = v_row * kD + (((lane >> 4) ^ (kD == 128 ? (v_row & 7) : ((v_row >> 1) & 3))) << 4);
   for (int k = 0; k < n_steps; ++k) {
-    if (!aborted && !mbar_wait(smem_u32(&sm.full[w][st]), ph, p.err)) aborted = true;
-    aborted = __any_sync(0xffffffffu, aborted);
-    const Step s = sm.step[w][st];
+    const Step s = sm.step[warp][k & 1];  // written by this warp
     const bool ring = s.flags & kRingStep, empty = s.flags & kEmpty;
-    const int h = head_of(s.sub), n0 = (s.sub - h * p.row_tiles) * kRows + 8 * kNT * wr;  // this warp's rows
+    if (!aborted && !mbar_wait(smem_u32(&sm.k_full[warp]), k & 1, p.err)) aborted = true;
     if (s.flags & kFirst) {
+      const int h = head_of(s.sub), n0 = (s.sub - h * p.row_tiles) * kRows;
       begins = s.flags & kBegin;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
@@ -528,11 +549,10 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
         // queries: fp16 fragments, k index permuted as the codes' ldmatrix gives it
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
-          const int n = min(n0 + 8 * nt + g, p.rows - 1), tok = token_of(p, n);
-          const uint16_t* row = p.q.row(s.b, h * p.group + n - tok * p.group, tok) + 4 * t;
-          uint2 raw[kChunks];
+          uint2 raw[kChunks];  // (rows that do not exist hold anything; nothing of them is stored)
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c) raw[c] = __ldg(reinterpret_cast<const uint2*>(row + 16 * c));
+          for (int c = 0; c < kChunks; ++c)
+            raw[c] = *reinterpret_cast<const uint2*>(&sm.q[warp][8 * nt + g][32 * c + 8 * t]);
           float top = 0.f;
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
@@ -549,244 +569,267 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
 #pragma unroll
           for (int c = 0; c < kChunks; ++c) {
             const float2 a = Elem<kBf16>::unpack(raw[c].x), b = Elem<kBf16>::unpack(raw[c].y);
-            qf[nt][c][0] = pack_half2(a.x * f, a.y * f);
-            qf[nt][c][1] = pack_half2(b.x * f, b.y * f);
+            const uint32_t lo = pack_half2(a.x * f, a.y * f), hi = pack_half2(b.x * f, b.y * f);
+            if constexpr (H::kQShared)
+              *reinterpret_cast<uint2*>(&sm.q[warp][8 * nt + g][32 * c + 8 * t]) = make_uint2(lo, hi);
+            else
+              qf[nt][c][0] = lo, qf[nt][c][1] = hi;
           }
           qscale[nt][0] = __shfl_sync(0xffffffffu, back, 8 * t);      // from a lane of row 2t
           qscale[nt][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);  // and of 2t + 1
         }
       }
     }
+    auto q_frag = [&](int nt, int c, uint32_t& b0, uint32_t& b1) {  // (a lane reads what it wrote)
+      if constexpr (H::kQShared)
+        lds8(q_at + nt * 8 * H::kQStride + 32 * c, b0, b1);
+      else
+        b0 = qf[nt][c][0], b1 = qf[nt][c][1];
+    };
+    const uint32_t kb = smem_u32(sm.stage[warp]), vb = kb + G::kHalf;
+    const int n_tok = s.flags >> 8;  // of a ring step
+    const int rounds = ring ? (n_tok + H::kTok - 1) / H::kTok : kRounds;
 
-    if (!empty) {
-      const uint32_t kb = smem_u32(sm.stage[w][st]), vb = kb + kHalf;
-      // ---- scores, S^T: token g (0, 1), g + 8 (2, 3); rows 2t, 2t + 1
+#pragma unroll 1
+    for (int round = 0; round < rounds; ++round) {
       float sc[kTC][kNT][4];
+      if (!empty) {
+        // ---- scores, S^T: rows g (0, 1) and g + 8 (2, 3) of 16 tokens; query rows 2t, 2t + 1
+        if (!ring) {
+          const uint32_t ka = kb + k_off + round * H::kTok * kD;
 #pragma unroll
-      for (int i = 0; i < kTC; ++i)
+          for (int c = 0; c < kChunks; c += 2) {
+            const uint32_t kc = ka ^ (c << 4);  // (its column is below the row's 128 or 64 bytes)
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
+            for (int i = 0; i < kTC; ++i) {
+              uint32_t r[4];
+              ldmatrix_x4(kc + 16 * i * kD, r[0], r[1], r[2], r[3]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[i][nt][e] = 0.f;
-      if (!ring) {
+              for (int j = 0; j < 2; ++j) {
+                uint32_t a0, a1, a2, a3;
+                to_half<kInt8>(r[2 * j], a0, a2);
+                to_half<kInt8>(r[2 * j + 1], a1, a3);
 #pragma unroll
-        for (int c = 0; c < kChunks; c += 2)
+                for (int nt = 0; nt < kNT; ++nt) {
+                  uint32_t b0, b1;
+                  q_frag(nt, c + j, b0, b1);
+                  if (c + j == 0)
+                    mma_first(sc[i][nt], a0, a1, a2, a3, b0, b1);
+                  else
+                    mma_16816(sc[i][nt], a0, a1, a2, a3, b0, b1);
+                }
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kTC; ++i)
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[i][nt][e] = 0.f;
+#pragma unroll
+          for (int i = 0; i < kRC; ++i) {
+            const int tok0 = round * H::kTok + 16 * i;
+            if (tok0 >= n_tok) break;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              // row & 7 == g for both of this lane's rows
+              const uint32_t at = kb + (c >> 2) * G::kRegion + (tok0 + g) * 128 +
+                                  ((((c & 3) * 2 + (t >> 1)) ^ g) << 4) + (t & 1) * 8;
+              uint32_t a0, a1, a2, a3;
+              lds8(at, a0, a2);
+              lds8(at + 8 * 128, a1, a3);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                uint32_t b0, b1;
+                q_frag(nt, c, b0, b1);
+                if constexpr (kBf16) b0 = half_to_bf16(b0), b1 = half_to_bf16(b1);
+                mma_elem<kBf16>(sc[i][nt], a0, a1, a2, a3, b0, b1);
+              }
+            }
+          }
+        }
+      }
+      if (round == rounds - 1) {
+        if constexpr (H::kQShared) fence_proxy_async_smem();  // fragments stored there; a bulk copy may follow
+        __syncwarp();
+        issue(k + 1, false);
+      }
+      if (!empty) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          const float f0 = s.ks * qscale[nt][0], f1 = s.ks * qscale[nt][1];
+#pragma unroll
+          for (int i = 0; i < kTC; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[i][nt][e] *= (e & 1) ? f1 : f0;
+        }
+        if (s.flags & kMasked) {  // (a ring step is)
+          const int pos0 = s.pos0 + round * H::kTok, hi = ring ? 8 + g : 8 + (g ^ 4);
+#pragma unroll
+          for (int i = 0; i < kTC; ++i)
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if ((ring && i >= kRC) || !sees(p, pos0 + 16 * i + (e < 2 ? g : hi), limit[nt][e & 1]))
+                  sc[i][nt][e] = -INFINITY;
+        }
+        // ---- online softmax, and P as B fragments
+        float alpha[kNT][2], row_vs[kNT][2];
+        uint32_t pb[kTC][kNT][2], pl[kTC][kNT][2];
+        bool moved = false;
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          float ref[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < kTC; ++i) x = fmaxf(x, fmaxf(sc[i][nt][e], sc[i][nt][2 + e]));
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+            // a row that sees nothing of this block takes nothing of it, not even a scale that is NaN
+            row_vs[nt][e] = x == -INFINITY ? 0.f : s.vs;
+            const float mn = fmaxf(m[nt][e], x);
+            ref[e] = mn == -INFINITY ? 0.f : mn;
+            alpha[nt][e] = fast_exp2(m[nt][e] - ref[e]);
+            moved |= alpha[nt][e] != 1.f;
+            m[nt][e] = mn;
+            l[nt][e] *= alpha[nt][e];
+          }
 #pragma unroll
           for (int i = 0; i < kTC; ++i) {
-            const uint32_t row = 16 * i + ((lane >> 3) & 1) * 8 + (lane & 7);
-            const uint32_t chunk = (c + (lane >> 4)) ^ (kD == 128 ? (row & 7) : ((row >> 1) & 3));
-            uint32_t r[4];
-            ldmatrix_x4(kb + row * kD + chunk * 16, r[0], r[1], r[2], r[3]);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t a0, a1, a2, a3;
-              to_half<kInt8, false>(r[2 * j], a0, a2);
-              to_half<kInt8, false>(r[2 * j + 1], a1, a3);
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt)
-                mma_16816(sc[i][nt], a0, a1, a2, a3, qf[nt][c + j][0], qf[nt][c + j][1]);
+            const float p0 = fast_exp2(sc[i][nt][0] - ref[0]), p1 = fast_exp2(sc[i][nt][1] - ref[1]);
+            const float p2 = fast_exp2(sc[i][nt][2] - ref[0]), p3 = fast_exp2(sc[i][nt][3] - ref[1]);
+            l[nt][0] += p0 + p2;
+            l[nt][1] += p1 + p3;
+            uint32_t hi0, hi1, lo0 = 0, lo1 = 0;
+            if (kBf16 && ring) {
+              split_pair<true>(p0, p1, hi0, lo0);
+              split_pair<true>(p2, p3, hi1, lo1);
+            } else if (kSplitP) {
+              split_pair<false>(p0, p1, hi0, lo0);
+              split_pair<false>(p2, p3, hi1, lo1);
+            } else {
+              hi0 = pack_half2(p0, p1);
+              hi1 = pack_half2(p2, p3);
+            }
+            pb[i][nt][0] = movmatrix_trans(hi0);  // rows 2t, 2t + 1 of the tokens, query row g
+            pb[i][nt][1] = movmatrix_trans(hi1);  // and 2t + 8, 2t + 9
+            if (kSplitP || (ring && i < kRC)) {
+              pl[i][nt][0] = movmatrix_trans(lo0);
+              pl[i][nt][1] = movmatrix_trans(lo1);
             }
           }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kRC; ++i)
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            // row & 7 == g for both of this lane's rows
-            const uint32_t at = kb + (c >> 2) * G::kRegion + (16 * i + g) * 128 +
-                                ((((c & 3) * 2 + (t >> 1)) ^ g) << 4) + (t & 1) * 8;
-            uint32_t a0, a1, a2, a3;
-            lds8(at, a0, a2);
-            lds8(at + 8 * 128, a1, a3);
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-              uint32_t b0 = qf[nt][c][0], b1 = qf[nt][c][1];
-              if constexpr (kBf16) b0 = half_to_bf16(b0), b1 = half_to_bf16(b1);
-              mma_elem<kBf16>(sc[i][nt], a0, a1, a2, a3, b0, b1);
-            }
-          }
-      }
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        const float f0 = s.ks * qscale[nt][0], f1 = s.ks * qscale[nt][1];
-#pragma unroll
-        for (int i = 0; i < kTC; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[i][nt][e] *= (e & 1) ? f1 : f0;
-      }
-      if (s.flags & kMasked) {
-#pragma unroll
-        for (int i = 0; i < kTC; ++i)
+        }
+        if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
           for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if ((ring && i >= kRC) || !sees(p, s.pos0 + 16 * i + g + (e >> 1) * 8, limit[nt][e & 1]))
-                sc[i][nt][e] = -INFINITY;
-      }
-      // ---- online softmax, and P as B fragments
-      float alpha[kNT][2], row_vs[kNT][2];
-      uint32_t pb[kTC][kNT][2], pl[kTC][kNT][2];
-      bool moved = false;
+            for (int c = 0; c < kChunks; ++c)
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        float ref[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float x = -INFINITY;
-#pragma unroll
-          for (int i = 0; i < kTC; ++i) x = fmaxf(x, fmaxf(sc[i][nt][e], sc[i][nt][2 + e]));
-#pragma unroll
-          for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-          // a row that sees nothing of this block takes nothing of it, not even a scale that is NaN
-          row_vs[nt][e] = x == -INFINITY ? 0.f : s.vs;
-          const float mn = fmaxf(m[nt][e], x);
-          ref[e] = mn == -INFINITY ? 0.f : mn;
-          alpha[nt][e] = fast_exp2(m[nt][e] - ref[e]);
-          moved |= alpha[nt][e] != 1.f;
-          m[nt][e] = mn;
-          l[nt][e] *= alpha[nt][e];
+              for (int e = 0; e < 4; ++e) acc[nt][c][e] *= alpha[nt][e & 1];
         }
+        // ---- O^T += vs V^T P^T
+        if (round == 0 && !aborted && !mbar_wait(smem_u32(&sm.v_full[warp]), k & 1, p.err)) aborted = true;
+        if (!ring) {
+          const uint32_t va = vb + v_off + round * H::kTok * kD;
 #pragma unroll
-        for (int i = 0; i < kTC; ++i) {
-          const float p0 = fast_exp2(sc[i][nt][0] - ref[0]), p1 = fast_exp2(sc[i][nt][1] - ref[1]);
-          const float p2 = fast_exp2(sc[i][nt][2] - ref[0]), p3 = fast_exp2(sc[i][nt][3] - ref[1]);
-          l[nt][0] += p0 + p2;
-          l[nt][1] += p1 + p3;
-          uint32_t lo0 = 0, lo1 = 0;
-          if (kBf16 && ring) {
-            split_pair<true>(p0, p1, pb[i][nt][0], lo0);
-            split_pair<true>(p2, p3, pb[i][nt][1], lo1);
-          } else if (kSplitP) {
-            split_pair<false>(p0, p1, pb[i][nt][0], lo0);
-            split_pair<false>(p2, p3, pb[i][nt][1], lo1);
-          } else {
-            pb[i][nt][0] = pack_half2(p0, p1);
-            pb[i][nt][1] = pack_half2(p2, p3);
-          }
-          pb[i][nt][0] = movmatrix_trans(pb[i][nt][0]);  // tokens 2t, 2t + 1 of row g
-          pb[i][nt][1] = movmatrix_trans(pb[i][nt][1]);  // and 2t + 8, 2t + 9
-          if (kSplitP || ring) {
-            pl[i][nt][0] = movmatrix_trans(lo0);
-            pl[i][nt][1] = movmatrix_trans(lo1);
-          }
-        }
-      }
-      if (__any_sync(0xffffffffu, moved)) {
+          for (int c = 0; c < kChunks; c += 2) {
+            const uint32_t vc = va ^ (c << 4);
+            float blk[2][kNT][4];
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
+            for (int i = 0; i < kTC; ++i) {
+              uint32_t r[4];
+              ldmatrix_b8_trans(vc + 16 * i * kD, r[0], r[1], r[2], r[3]);
 #pragma unroll
-          for (int c = 0; c < kChunks; ++c)
+              for (int j = 0; j < 2; ++j) {
+                uint32_t a0, a1, a2, a3;
+                to_half<kInt8>(r[2 * j], a0, a2);
+                to_half<kInt8>(r[2 * j + 1], a1, a3);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[nt][c][e] *= alpha[nt][e & 1];
-      }
-      // ---- O^T += vs V^T P^T
-      if (!ring) {
-#pragma unroll
-        for (int c = 0; c < kChunks; c += 2) {
-          float blk[2][kNT][4];
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) blk[j][nt][e] = 0.f;
-#pragma unroll
-          for (int i = 0; i < kTC; ++i) {
-            const uint32_t row = 16 * i + ((lane >> 3) & 1) * 8 + (lane & 7);
-            const uint32_t chunk = (c + (lane >> 4)) ^ (kD == 128 ? (row & 7) : ((row >> 1) & 3));
-            uint32_t r[4];
-            ldmatrix_x4_trans(vb + row * kD + chunk * 16, r[0], r[1], r[2], r[3]);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              uint32_t a0, a1, a2, a3;
-              to_half<kInt8, true>(r[2 * j], a0, a1);
-              to_half<kInt8, true>(r[2 * j + 1], a2, a3);
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-                mma_16816(blk[j][nt], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
-                if constexpr (kSplitP) mma_16816(blk[j][nt], a0, a1, a2, a3, pl[i][nt][0], pl[i][nt][1]);
-              }
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) acc[nt][c + j][e] += row_vs[nt][e & 1] * blk[j][nt][e];
-        }
-      } else {
-        const int n_tok = s.flags >> 8;
-        for (int i = 0; i < kRC && 16 * i < n_tok; ++i) {
-          // (selects instead of a variable index: the fragments stay in registers)
-          uint32_t b0[kNT], b1[kNT], c0[kNT], c1[kNT];
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            b0[nt] = i ? pb[kRC - 1][nt][0] : pb[0][nt][0], b1[nt] = i ? pb[kRC - 1][nt][1] : pb[0][nt][1];
-            c0[nt] = i ? pl[kRC - 1][nt][0] : pl[0][nt][0], c1[nt] = i ? pl[kRC - 1][nt][1] : pl[0][nt][1];
-          }
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c) {
-            uint32_t v[4], a[4], bad = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {  // tokens 2t, 2t + 1, 2t + 8, 2t + 9: dims 2g, 2g + 1
-              const uint32_t row = 16 * i + 2 * t + (e & 1) + (e >> 1) * 8;
-              v[e] = lds4(vb + (c >> 2) * G::kRegion + row * 128 + ((((c & 3) * 2 + (g >> 2)) ^ (row & 7)) << 4) +
-                          (g & 3) * 4);
-              if (static_cast<int>(row) >= n_tok) v[e] = 0u;  // no token: whatever the slot held
-              bad |= nonfinite_mask<kBf16>(v[e]);
-            }
-            a[0] = __byte_perm(v[0], v[1], 0x5410);
-            a[1] = __byte_perm(v[0], v[1], 0x7632);
-            a[2] = __byte_perm(v[2], v[3], 0x5410);
-            a[3] = __byte_perm(v[2], v[3], 0x7632);
-            if (__any_sync(0xffffffffu, bad != 0)) {
-              // Values that are not finite would reach rows that do not see
-              // them (0 * NaN).  They are taken out, and a product of their
-              // places with the rows' masks says which sums they make NaN.
-              const uint32_t one = kBf16 ? 0x3f803f80u : 0x3c003c00u;
-              uint32_t at[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const uint32_t mk = nonfinite_mask<kBf16>(a[e]);
-                at[e] = one & mk;
-                a[e] &= ~mk;
-              }
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-                const int lim = limit_at(s.len, s.cnt, n0 + 8 * nt + g);
-                uint32_t see[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int pos = s.pos0 + 16 * i + 2 * t + 8 * e;
-                  see[e] = one & ((sees(p, pos, lim) ? 0xffffu : 0u) | (sees(p, pos + 1, lim) ? 0xffff0000u : 0u));
+                for (int nt = 0; nt < kNT; ++nt) {
+                  if (i == 0)
+                    mma_first(blk[j][nt], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
+                  else
+                    mma_16816(blk[j][nt], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
+                  if constexpr (kSplitP) mma_16816(blk[j][nt], a0, a1, a2, a3, pl[i][nt][0], pl[i][nt][1]);
                 }
-                float hit[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_elem<kBf16>(hit, at[0], at[1], at[2], at[3], see[0], see[1]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (hit[e] > 0.f) acc[nt][c][e] = NAN;
               }
             }
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt) {
-              mma_elem<kBf16>(acc[nt][c], a[0], a[1], a[2], a[3], b0[nt], b1[nt]);
-              mma_elem<kBf16>(acc[nt][c], a[0], a[1], a[2], a[3], c0[nt], c1[nt]);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][c + j][e] += row_vs[nt][e & 1] * blk[j][nt][e];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kRC; ++i) {
+            const int tok0 = round * H::kTok + 16 * i;
+            if (tok0 >= n_tok) break;
+            // halves of a register are tokens 2t and 2t + 1 (a0, a1) or 2t + 8 and 2t + 9 (a2, a3); where there is
+            // no token, whatever the slot held is taken out
+            auto keep = [&](int tok) { return (tok < n_tok ? 0xffffu : 0u) | (tok + 1 < n_tok ? 0xffff0000u : 0u); };
+            const uint32_t keep0 = keep(tok0 + 2 * t), keep1 = keep(tok0 + 2 * t + 8);
+            const uint32_t row = tok0 + (lane >> 4) * 8 + (lane & 7);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c) {
+              uint32_t a[4];
+              ldmatrix_x4_trans(vb + (c >> 2) * G::kRegion + row * 128 +
+                                    ((((c & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4),
+                                a[0], a[1], a[2], a[3]);
+              a[0] &= keep0, a[1] &= keep0, a[2] &= keep1, a[3] &= keep1;
+              const uint32_t bad = nonfinite_mask<kBf16>(a[0]) | nonfinite_mask<kBf16>(a[1]) |
+                                   nonfinite_mask<kBf16>(a[2]) | nonfinite_mask<kBf16>(a[3]);
+              if (__any_sync(0xffffffffu, bad != 0)) {
+                // Values that are not finite would reach rows that do not see
+                // them (0 * NaN).  They are taken out, and a product of their
+                // places with the rows' masks says which sums they make NaN.
+                const int h = head_of(s.sub), n0 = (s.sub - h * p.row_tiles) * kRows;
+                const uint32_t one = kBf16 ? 0x3f803f80u : 0x3c003c00u;
+                uint32_t at[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t mk = nonfinite_mask<kBf16>(a[e]);
+                  at[e] = one & mk;
+                  a[e] &= ~mk;
+                }
+#pragma unroll
+                for (int nt = 0; nt < kNT; ++nt) {
+                  const int lim = limit_at(s.len, s.cnt, n0 + 8 * nt + g);
+                  uint32_t see[2];
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const int pos = s.pos0 + tok0 + 2 * t + 8 * e;
+                    see[e] = one & ((sees(p, pos, lim) ? 0xffffu : 0u) | (sees(p, pos + 1, lim) ? 0xffff0000u : 0u));
+                  }
+                  float hit[4] = {0.f, 0.f, 0.f, 0.f};
+                  mma_elem<kBf16>(hit, at[0], at[1], at[2], at[3], see[0], see[1]);
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    if (hit[e] > 0.f) acc[nt][c][e] = NAN;
+                }
+              }
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                mma_elem<kBf16>(acc[nt][c], a[0], a[1], a[2], a[3], pb[i][nt][0], pb[i][nt][1]);
+                mma_elem<kBf16>(acc[nt][c], a[0], a[1], a[2], a[3], pl[i][nt][0], pl[i][nt][1]);
+              }
             }
           }
         }
       }
     }
     __syncwarp();
-    if (kR > 1 && lane == 0) mbar_arrive(smem_u32(&sm.empty[w][st]));
-    if (++st == kStages) st = 0, ph ^= 1;
-    // one warp refills the stage it has just read; with several, the one before,
-    // which the others have most likely left
-    if (wr == 0) issue_to(kR == 1 ? k + 1 + kStages : k + kStages);
+    issue(k + 1, true);
 
     if (!(s.flags & kLast)) continue;
     // ---- end of the piece
+    const int h = head_of(s.sub), n0 = (s.sub - h * p.row_tiles) * kRows;
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
@@ -795,45 +838,54 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
         for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
     if (begins && (s.flags & kEnd)) {
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
+      for (int nt = 0; nt < kNT; ++nt) {
+        float inv[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int n = n0 + 8 * nt + 2 * t + e;
-          if (n >= p.rows) continue;
-          const int tok = token_of(p, n);
-          const float inv = (l[nt][e] == 0.f || tok >= s.cnt) ? 0.f : 1.f / l[nt][e];
-          uint16_t* out = p.o.row(s.b, h * p.group + n - tok * p.group, tok) + 2 * g;
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c)
-            *reinterpret_cast<uint32_t*>(out + 16 * c) =
-                inv == 0.f ? 0u : Elem<kBf16>::pack(acc[nt][c][e] * inv, acc[nt][c][2 + e] * inv);
+          const int tok = token_of(p, min(n0 + 8 * nt + 2 * t + e, p.rows - 1));
+          inv[e] = (l[nt][e] == 0.f || tok >= s.cnt) ? 0.f : 1.f / l[nt][e];
         }
+        // dims g of rows 2t, 2t + 1 become dims 2t, 2t + 1 of row g
+        const int n = n0 + 8 * nt + g, tok = token_of(p, min(n, p.rows - 1));
+        uint16_t* out = p.o.row(s.b, h * p.group + n - tok * p.group, tok) + 2 * t;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; e += 2) {
+            const uint32_t x = movmatrix_trans(
+                Elem<kBf16>::pack(inv[0] == 0.f ? 0.f : acc[nt][c][e] * inv[0],
+                                  inv[1] == 0.f ? 0.f : acc[nt][c][e + 1] * inv[1]));
+            if (n < p.rows) *reinterpret_cast<uint32_t*>(out + 16 * c + 4 * e) = x;
+          }
+      }
       continue;
     }
-    // a part of a unit: left for the CTA's end
-    // (in its stages where one warp has done its last step)
-    float* data = kR == 1 && k == n_steps - 1 ? reinterpret_cast<float*>(sm.stage[w])
-                                              : p.partials + (int64_t(worker) * 2 + (begins ? 1 : 0)) * kPiece;
-    if (wr == 0 && lane == 0)
-      sm.part[w][begins ? 1 : 0] = Part{static_cast<int>(x0) + k - s.step, data, s.b, s.sub, s.cnt, s.steps,
-                                        kFirst | (begins ? kBegin : 0) | (s.flags & kEnd)};
+    // a part of a unit: left for the CTA's end (in the worker's stages after its last step, where it fits)
+    constexpr bool kFits = kPiece * 4 <= sizeof(sm.stage[0]);
+    float* data = kFits && k == n_steps - 1 ? reinterpret_cast<float*>(sm.stage[warp])
+                                   : p.partials + (int64_t(worker) * 2 + (begins ? 1 : 0)) * kPiece;
+    if (lane == 0)
+      sm.part[warp][begins ? 1 : 0] = Part{static_cast<int>(x0) + k - s.step, data, s.b, s.sub, s.cnt, s.steps,
+                                           kFirst | (begins ? kBegin : 0) | (s.flags & kEnd)};
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = 8 * kNT * wr + 8 * nt + 2 * t + e;
+        const int r = 8 * nt + 2 * t + e;
         if (g == 0) reinterpret_cast<float2*>(data)[r] = make_float2(m[nt][e], l[nt][e]);
-        float* o = data + 2 * kRows + r * kD + 2 * g;
+        float* o = data + 2 * kRows + r * kD + g;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-          *reinterpret_cast<float2*>(o + 16 * c) = make_float2(acc[nt][c][e], acc[nt][c][2 + e]);
+        for (int c = 0; c < kChunks; ++c) {
+          o[16 * c] = acc[nt][c][e];
+          o[16 * c + 8] = acc[nt][c][2 + e];
+        }
       }
   }
 
   // ---- cut units.  The CTA's parts in order (entry 2w + slot: slot 0 goes on
   // from the worker before, slot 1 begins a unit) form runs, one per unit.
   __syncthreads();
-  const int e_flags = lane < 2 * kWorkers ? sm.part[lane >> 1][lane & 1].flags : 0;
+  const int e_flags = lane < 2 * H::kWarps ? sm.part[lane >> 1][lane & 1].flags : 0;
   const uint32_t valid = __ballot_sync(0xffffffffu, e_flags != 0);
   if (valid == 0) return;
   const uint32_t begin_mask = __ballot_sync(0xffffffffu, e_flags & kBegin), end_mask = __ballot_sync(0xffffffffu, e_flags & kEnd);
@@ -849,7 +901,7 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
     for (int k = 0; k < kCols; k += 2)
       *reinterpret_cast<uint32_t*>(out + k) = inv == 0.f ? 0u : Elem<kBf16>::pack(a[k] * inv, a[k + 1] * inv);
   };
-  float* const cta_parts = p.partials + int64_t(gridDim.x) * kWorkers * 2 * kPiece;
+  float* const cta_parts = p.partials + int64_t(gridDim.x) * H::kWarps * 2 * kPiece;
   int cut[2] = {-1, -1};  // first entries of the runs that other CTAs share: going on from one, and begun here
   int task = 0;
   for (uint32_t left = run_starts; left; left &= left - 1) {
@@ -881,7 +933,7 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
   if (cut[0] < 0 && cut[1] < 0) return;
   __threadfence();
   __syncthreads();
-  auto cta_of = [&](int x) { return static_cast<int>(split.owner(x) / kWorkers); };
+  auto cta_of = [&](int x) { return static_cast<int>(split.owner(x) / H::kWarps); };
   if (tid < 2) {
     sm.last[tid] = 0;
     const int c = tid ? cut[1] : cut[0];
@@ -911,7 +963,7 @@ __global__ void __launch_bounds__(Shape<kNT, kR>::kThreads, 1)
 }
 
 struct Plan {
-  int nt, r, row_tiles, workers, n_ctas;
+  int nt, row_tiles, n_ctas;
   size_t bytes;
 };
 
@@ -920,29 +972,28 @@ int max_ctas() {
   return sms > 0 ? sms : 148;
 }
 
-// Query rows of a unit: up to 8 or 16 for one warp, 32 for two, 64 for four.
+// Query rows of a unit: up to 8, 16 or 32; more of them are further units.
 Plan plan(const nsa_kv8_cache* c, int64_t rows) {
   Plan s;
-  s.nt = rows <= 8 ? 1 : 2;
-  s.r = rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-  const int tile = 8 * s.nt * s.r;
+  s.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  const int tile = 8 * s.nt, workers = s.nt == 1 ? Shape<128, 1, true>::kWarps : Shape<128, 2, true>::kWarps;
   s.row_tiles = static_cast<int>((rows + tile - 1) / tile);
-  s.workers = (s.nt == 1 ? 12 : 8) / s.r;
-  const int64_t most = c->batch * c->n_kv_heads * s.row_tiles * (2 * c->max_blocks + 4);  // steps
-  const int64_t ctas = (most + s.workers - 1) / s.workers;
+  const int64_t most = c->batch * c->n_kv_heads * s.row_tiles * (c->max_blocks + 2);  // steps
+  const int64_t ctas = (most + workers - 1) / workers;
   s.n_ctas = static_cast<int>(ctas < max_ctas() ? ctas : max_ctas());
-  s.bytes = size_t(s.n_ctas) * (s.workers + 1) * 2 * tile * (2 + c->head_dim) * sizeof(float);
+  s.bytes = size_t(s.n_ctas) * (workers + 1) * 2 * tile * (2 + c->head_dim) * sizeof(float);
   return s;
 }
 
-template <int kD, int kNT, int kR, bool kBf16, bool kInt8>
+template <int kD, int kNT, bool kBf16, bool kInt8>
 int launch_attend(const Plan& plan, const CUtensorMap (&maps)[4], const AttendParams& p, cudaStream_t stream) {
-  using S = Smem<kNT, kR>;
-  using H = Shape<kNT, kR>;
-  static_assert(offsetof(S, stage) == 0 && offsetof(S, step) % 16 == 0, "TMA destinations, vector reads");
+  using S = Smem<kD, kNT, !kBf16>;
+  using H = Shape<kD, kNT, !kBf16>;
+  static_assert(offsetof(S, stage) == 0 && Geo<kD>::kHalf % 1024 == 0, "TMA destinations");
+  static_assert(offsetof(S, q) % 16 == 0 && offsetof(S, step) % 16 == 0, "vector reads");
   static_assert(sizeof(S) <= 227 * 1024, "shared memory of an SM");
-  static_assert(2 * H::kWorkers <= 32, "a lane for each part");
-  auto kernel = kv8_attend_kernel<kD, kNT, kR, kBf16, kInt8>;
+  static_assert(2 * H::kWarps <= 32, "a lane for each part");
+  auto kernel = kv8_attend_kernel<kD, kNT, kBf16, kInt8>;
   static bool attr_set[64] = {false};
   const int dev = current_device().device;
   if (dev < 0 || dev >= 64) return fail(NSA_ERR_CUDA, "no CUDA device");
@@ -959,10 +1010,9 @@ int launch_attend(const Plan& plan, const CUtensorMap (&maps)[4], const AttendPa
 
 template <int kD, bool kBf16, bool kInt8>
 int launch_rows(const Plan& s, const CUtensorMap (&maps)[4], const AttendParams& p, cudaStream_t stream) {
-  if (s.nt == 1) return launch_attend<kD, 1, 1, kBf16, kInt8>(s, maps, p, stream);
-  if (s.r == 1) return launch_attend<kD, 2, 1, kBf16, kInt8>(s, maps, p, stream);
-  if (s.r == 2) return launch_attend<kD, 2, 2, kBf16, kInt8>(s, maps, p, stream);
-  return launch_attend<kD, 2, 4, kBf16, kInt8>(s, maps, p, stream);
+  if (s.nt == 1) return launch_attend<kD, 1, kBf16, kInt8>(s, maps, p, stream);
+  if (s.nt == 2) return launch_attend<kD, 2, kBf16, kInt8>(s, maps, p, stream);
+  return launch_attend<kD, 4, kBf16, kInt8>(s, maps, p, stream);
 }
 
 int check_shape(const nsa_kv8_cache* cache, int64_t n_heads, int64_t n_tokens) {
@@ -1009,7 +1059,7 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
   p.n_tokens = static_cast<int>(n_tokens);
   p.rows = p.group * p.n_tokens;
   const kv8::Plan s = kv8::plan(cache, p.rows);
-  if (int64_t(p.c.n_kv_heads) * s.row_tiles * (2 * int64_t(p.c.max_blocks) + 4) > 0x7fffffff)
+  if (int64_t(p.c.n_kv_heads) * s.row_tiles * (int64_t(p.c.max_blocks) + 2) > 0x7fffffff)
     return fail(NSA_ERR_UNSUPPORTED, "too many (head, block) pairs in a sequence");
   if (!workspace || workspace_bytes < s.bytes)
     return fail(NSA_ERR_WORKSPACE, "workspace of %zu bytes required (got %zu)", s.bytes, workspace ? workspace_bytes : size_t(0));
@@ -1030,7 +1080,7 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
   const uint64_t code_dims[2] = {d, static_cast<uint64_t>(p.c.n_pages) * p.c.n_kv_heads * kv8::kBlock};
   const uint64_t ring_dims[2] = {d, static_cast<uint64_t>(p.c.batch) * p.c.n_kv_heads * kv8::kRing};
   const uint64_t code_stride[1] = {d}, ring_stride[1] = {2 * d};
-  const uint32_t code_box[2] = {static_cast<uint32_t>(d), static_cast<uint32_t>(4096 / d)}, ring_box[2] = {64, 8};
+  const uint32_t code_box[2] = {static_cast<uint32_t>(d), kv8::kBlock}, ring_box[2] = {64, 8};
   const CUtensorMapSwizzle swz = d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   CUtensorMap maps[4];
   const void* base[4] = {p.c.k_codes, p.c.v_codes, p.c.k_ring, p.c.v_ring};
