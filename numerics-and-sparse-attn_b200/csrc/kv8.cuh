@@ -24,6 +24,7 @@ struct Cache {
   uint16_t *k_ring, *v_ring;
   int64_t* lens;
   int64_t* ring_floor;
+  int32_t* unclean;
   int32_t* tickets;
 };
 

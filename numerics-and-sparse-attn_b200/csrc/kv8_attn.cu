@@ -33,6 +33,8 @@ namespace nsa {
 namespace kv8 {
 namespace {
 
+constexpr int kShare = 6;   // steps of a CTA at least, where there are more CTAs than units
+constexpr int kWhole = 32;  // steps of a unit that is not cut between CTAs
 constexpr int kLensCached = 512;  // sequence lengths kept in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -102,15 +104,15 @@ __device__ __forceinline__ int2 load_len(const AttendParams& p, int b) {
   return make_int2(static_cast<int>(len), static_cast<int>(cnt));
 }
 
-// What a worker has to know of a staged step.
-struct alignas(16) Step {
+// What a worker has to know of a step.
+struct Step {
   int b, sub;    // sequence; KV head * row_tiles + row tile
-  int pos0;      // position of its first token
-  int flags;     // kFirst..., and from bit 8 on the tokens of a ring step
   int len, cnt;  // of the sequence
-  int step, steps;  // of its unit
+  int pos0;      // position of its first token
+  int flags;     // kFirst..., and from bit 16 on the tokens of a ring step
+  int step, steps;  // which of its unit's
   float ks, vs;  // scales
-  int pad[2];
+  int row;       // of the tensor map
 };
 enum : int {
   kFirst = 1,   // of the worker's piece
@@ -119,7 +121,8 @@ enum : int {
   kEnd = 8,
   kRingStep = 16,
   kEmpty = 32,
-  kMasked = 64  // some row does not see some of its tokens
+  kMasked = 64,  // some row does not see some of its tokens
+  kUnclean = 128  // the ring may hold values that are not finite
 };
 
 // A worker's part of a cut unit.
@@ -139,9 +142,8 @@ struct Shape {
   static constexpr int kWarps = kNT == 1 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kRows = 8 * kNT;  // of a unit
-  static constexpr bool kQShared = kNT == 4;
   static constexpr int kQStride = kD * 2 + 32;  // bytes: rows 8 banks apart
-  static constexpr int kTok = kNT == 4 ? 16 : kNT == 2 || kSplit ? 32 : 64;  // tokens of a round of scores, softmax and sums
+  static constexpr int kTok = kNT == 4 ? 16 : 32;  // tokens of a round of scores, softmax and sums
 };
 
 template <int kD, int kNT, bool kSplit>
@@ -149,11 +151,11 @@ struct Smem {
   using H = Shape<kD, kNT, kSplit>;
   uint8_t stage[H::kWarps][2 * Geo<kD>::kHalf];  // K, V; 1024-aligned: TMA destinations
   uint8_t q[H::kWarps][H::kRows][H::kQStride];
-  Step step[H::kWarps][2];
   Part part[H::kWarps][2];
   int2 lens[kLensCached];
   int scan[H::kWarps];
   int before[H::kThreads];  // steps before a thread's sequences
+  int range[2];  // the CTA's steps
   int last[2];  // whether this CTA was the last of its first / last cut unit
   uint64_t k_full[H::kWarps], v_full[H::kWarps];
 };
@@ -243,15 +245,15 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
   lo = Elem<kBf16>::pack(x - back.x, y - back.y);
 }
 
-// The even split of `total` steps over n workers: the first `rem` take one
-// step more than the others.
+// The even split of `total` > 0 steps over at most `most` takers: the first
+// `rem` of n take one step more than the others, and takers from n on nothing.
 struct Split {
   uint32_t total, n, each, rem;
-  __device__ __forceinline__ Split(uint32_t total_, uint32_t workers) : total(total_), n(min(workers, total_)) {
+  __device__ __forceinline__ Split(uint32_t total_, uint32_t most) : total(total_), n(min(most, total_)) {
     each = total / n;
     rem = total - each * n;
   }
-  __device__ __forceinline__ uint32_t begin(uint32_t g) const { return g * each + min(g, rem); }
+  __device__ __forceinline__ uint32_t begin(uint32_t g) const { return g < n ? g * each + min(g, rem) : total; }
   __device__ __forceinline__ uint32_t owner(uint32_t x) const {
     const uint32_t wide = rem * (each + 1);
     return x < wide ? x / (each + 1) : rem + (x - wide) / each;
@@ -322,6 +324,7 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
   constexpr int kRounds = kBlock / H::kTok;
   constexpr int kRC = kTC < kRingTok / 16 ? kTC : kRingTok / 16;  // of a round of a ring step
   constexpr int kPiece = kRows * (2 + kD);      // floats of a partial result
+  constexpr int kKUnroll = 2;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   grid_launch_dependents();
   if (smem_u32(smem_raw) & 1023u) {
@@ -371,34 +374,61 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
     if (tid == 0) set_error(p.err, NSA_ERR_INVALID);
     return;
   }
-  const Split split(static_cast<uint32_t>(sum) * units, gridDim.x * H::kWarps);
-  if (blockIdx.x * H::kWarps >= split.n) return;  // the whole CTA has nothing to do
-  const uint32_t worker = blockIdx.x * H::kWarps + warp;
-  const uint32_t x0 = worker < split.n ? split.begin(worker) : split.total;
-  const int n_steps = worker < split.n ? static_cast<int>(split.begin(worker + 1) - x0) : 0;
   sm.before[tid] = before + prior - mine;
   __syncthreads();
+  // The sequence that holds step x: the last one that begins at it or before.
+  const int threads = (batch + per - 1) / per;
+  struct Found {
+    int b, begin, steps;  // the sequence's first step, and its steps a unit
+  };
+  auto find = [&](int x) {  // (a whole warp)
+    const int at = x / units;
+    int n = 0;
+    for (int i = lane; i < threads; i += 32) n += sm.before[i] <= at;
+    n = __reduce_add_sync(0xffffffffu, n) - 1;
+    Found f{n * per, sm.before[n], 0};
+    for (;;) {
+      const int2 l = f.b < kLensCached ? sm.lens[f.b] : load_len(p, f.b);
+      f.steps = make_seq(p, l.x, l.y).steps;
+      if (at < f.begin + f.steps) break;
+      f.begin += f.steps;
+      ++f.b;
+    }
+    f.begin *= units;
+    return f;
+  };
+  // a CTA for every kShare steps, or for every unit
+  const uint32_t total = static_cast<uint32_t>(sum) * units;
+  const Split split(total, min(gridDim.x, max((total + kShare - 1) / kShare, static_cast<uint32_t>(batch * units))));
+  if (blockIdx.x >= split.n) return;
+  // A CTA's range ends at unit borders where the unit there is short: a merge
+  // across CTAs costs as much as about kWhole steps of a CTA.
+  if (warp < 2) {
+    const uint32_t c = blockIdx.x + warp;
+    int x = split.begin(c);
+    if (x > 0 && c < split.n) {
+      const Found f = find(x);
+      const int in = (x - f.begin) % f.steps;
+      if (f.steps <= kWhole) x += 2 * in < f.steps ? -in : f.steps - in;
+    }
+    if (lane == 0) sm.range[warp] = x;
+  }
+  __syncthreads();
+  const int cta_steps = sm.range[1] - sm.range[0];
+  if (cta_steps == 0) return;  // the whole CTA
+  const Split shares(cta_steps, H::kWarps);  // (workers with steps are the first ones: their parts follow one another)
+  const int x0 = sm.range[0] + shares.begin(warp);
+  const int n_steps = sm.range[0] + shares.begin(warp + 1) - x0;
+  const uint32_t worker = blockIdx.x * H::kWarps + warp;
 
   // ---- issuing: lane i knows step batch0 + i
   int cur_b = 0, batch0 = -32;
   int cur_rel = 0;  // first step of sequence cur_b, from the worker's first
-  Step mystep{};
-  int myrow = 0;
-  if (n_steps > 0) {  // the sequence of the first step: the last one that begins at it or before
-    const int at = static_cast<int>(x0 / units), threads = (batch + per - 1) / per;
-    int n = 0;
-    for (int i = lane; i < threads; i += 32) n += sm.before[i] <= at;
-    n = __reduce_add_sync(0xffffffffu, n) - 1;
-    cur_b = n * per;
-    int begin = sm.before[n];
-    for (;;) {
-      const int2 l = cur_b < kLensCached ? sm.lens[cur_b] : load_len(p, cur_b);
-      const int steps = make_seq(p, l.x, l.y).steps;
-      if (at < begin + steps) break;
-      begin += steps;
-      ++cur_b;
-    }
-    cur_rel = begin * units - static_cast<int>(x0);
+  Step ahead{};
+  if (n_steps > 0) {
+    const Found f = find(x0);
+    cur_b = f.b;
+    cur_rel = f.begin - x0;
   }
   auto head_of = [&](int sub) { return p.row_tiles == 1 ? sub : sub / p.row_tiles; };
   auto limit_at = [&](int len, int cnt, int n) {
@@ -428,14 +458,14 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
     }
     if (k >= n_steps) return;
     const int h = head_of(sub), n0 = (sub - h * p.row_tiles) * kRows;
-    mystep.b = b;
-    mystep.sub = sub;
-    mystep.len = s.len;
-    mystep.cnt = s.cnt;
-    mystep.step = step;
-    mystep.steps = s.steps;
-    mystep.pos0 = 0;
-    mystep.ks = mystep.vs = 1.f;
+    ahead.b = b;
+    ahead.sub = sub;
+    ahead.len = s.len;
+    ahead.cnt = s.cnt;
+    ahead.step = step;
+    ahead.steps = s.steps;
+    ahead.pos0 = 0;
+    ahead.ks = ahead.vs = 1.f;
     int flags = (step == 0 ? kBegin | kFirst : 0) | (step == s.steps - 1 ? kEnd | kLast : 0);
     flags |= (k == 0 ? kFirst : 0) | (k == n_steps - 1 ? kLast : 0);
     const int blocks = s.sink_blocks + s.full - s.win_block;
@@ -451,66 +481,63 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
         set_error(p.err, NSA_ERR_INVALID);
         page = 0;
       }
-      mystep.ks = sc.x;
-      mystep.vs = sc.y;
-      mystep.pos0 = block * kBlock;
-      myrow = (page * p.c.n_kv_heads + h) * kBlock;
+      ahead.ks = sc.x;
+      ahead.vs = sc.y;
+      ahead.pos0 = block * kBlock;
+      ahead.row = (page * p.c.n_kv_heads + h) * kBlock;
       const int lo = limit_at(s.len, s.cnt, n0), hi = limit_at(s.len, s.cnt, n0 + kRows - 1);
-      if (mystep.pos0 + kBlock > lo || (p.window >= 0 && mystep.pos0 < hi - p.window && mystep.pos0 + kBlock > p.sink))
+      if (ahead.pos0 + kBlock > lo || (p.window >= 0 && ahead.pos0 < hi - p.window && ahead.pos0 + kBlock > p.sink))
         flags |= kMasked;
     } else {
-      mystep.pos0 = s.full * kBlock + (step - blocks) * kRingTok;
-      myrow = (b * p.c.n_kv_heads + h) * kRing + mystep.pos0 % kRing;
-      flags |= kRingStep | kMasked | (min(kRingTok, s.len - mystep.pos0) << 8);
+      ahead.pos0 = s.full * kBlock + (step - blocks) * kRingTok;
+      ahead.row = (b * p.c.n_kv_heads + h) * kRing + ahead.pos0 % kRing;
+      flags |= kRingStep | kMasked | (p.c.unclean[b] ? kUnclean : 0) | (min(kRingTok, s.len - ahead.pos0) << 16);
     }
-    mystep.flags = flags;
+    ahead.flags = flags;
   };
-  // Stages K (and with it the queries of a new piece and what is to be known of
-  // the step) or V of step k; called for k = 0, 1, ... in turn, K before V.
+  // Stages K (and with it the queries of a new piece) or V of step k; called for
+  // k = 0, 1, ... in turn, K before V.
+  int next_flags = 0, next_row = 0;
   auto issue = [&](int k, bool v) {
-    if (k < n_steps) {
-      if (!v && k >= batch0 + 32) fetch(k);
-      uint32_t q_rows = 0;
-      if (!v) {
-        const int flags = __shfl_sync(0xffffffffu, mystep.flags, k - batch0);
-        if ((flags & (kFirst | kEmpty)) == kFirst) {  // a query row a lane
-          const int b = __shfl_sync(0xffffffffu, mystep.b, k - batch0), sub = __shfl_sync(0xffffffffu, mystep.sub, k - batch0);
-          const int h = head_of(sub), n0 = (sub - h * p.row_tiles) * kRows;
-          q_rows = min(kRows, p.rows - n0);
-          if (lane < q_rows) {
-            const int n = n0 + lane, tok = token_of(p, n);
-            bulk_load(smem_u32(sm.q[warp][lane]), p.q.row(b, h * p.group + n - tok * p.group, tok), kD * 2,
-                      smem_u32(&sm.k_full[warp]));
-          }
+    if (k >= n_steps) return;
+    const uint32_t fb = smem_u32(v ? &sm.v_full[warp] : &sm.k_full[warp]);
+    uint32_t bytes = 0;
+    if (!v) {
+      if (k >= batch0 + 32) fetch(k);
+      next_flags = __shfl_sync(0xffffffffu, ahead.flags, k - batch0);
+      next_row = __shfl_sync(0xffffffffu, ahead.row, k - batch0);
+      if ((next_flags & (kFirst | kEmpty)) == kFirst) {  // a query row a lane
+        const int b = __shfl_sync(0xffffffffu, ahead.b, k - batch0), sub = __shfl_sync(0xffffffffu, ahead.sub, k - batch0);
+        const int h = head_of(sub), n0 = (sub - h * p.row_tiles) * kRows, n_rows = min(kRows, p.rows - n0);
+        fence_proxy_async_smem();  // the last piece's fragments were plain stores
+        __syncwarp();
+        if (lane < n_rows) {
+          const int n = n0 + lane, tok = token_of(p, n);
+          bulk_load(smem_u32(sm.q[warp][lane]), p.q.row(b, h * p.group + n - tok * p.group, tok), kD * 2, fb);
         }
+        bytes = n_rows * kD * 2;
       }
-      if (lane == k - batch0) {
-        const uint32_t fb = smem_u32(v ? &sm.v_full[warp] : &sm.k_full[warp]);
-        const uint32_t dst = smem_u32(sm.stage[warp]) + (v ? G::kHalf : 0);
-        uint32_t bytes = 0;
-        if (mystep.flags & kRingStep) {
-          const int boxes = ((mystep.flags >> 8) + 7) / 8;  // of 8 slots, those that hold tokens
-          bytes = boxes * 16 * kD;
-          for (int r = 0; r < boxes; ++r)
-            for (uint32_t c = 0; c < G::kRegions; ++c)
-              tma_load_2d(dst + c * G::kRegion + r * 1024, v ? &tm_vr : &tm_kr, fb, c * 64, myrow + 8 * r);
-        } else if (!(mystep.flags & kEmpty)) {
-          bytes = G::kHalf;
-          tma_load_2d(dst, v ? &tm_vc : &tm_kc, fb, 0, myrow);
-        }
-        // (the copies go first: the scales may still be on their way, and the phase ends with this arrival)
-        if (!v) sm.step[warp][k & 1] = mystep;
-        mbar_arrive_expect_tx(fb, bytes + q_rows * kD * 2);
+    }
+    const uint32_t dst = smem_u32(sm.stage[warp]) + (v ? G::kHalf : 0);
+    if (lane == 0) {
+      if (next_flags & kRingStep) {
+        const int boxes = ((next_flags >> 16) + 7) / 8;  // of 8 slots, those that hold tokens
+        mbar_arrive_expect_tx(fb, bytes + boxes * 16 * kD);
+        for (int r = 0; r < boxes; ++r)
+          for (uint32_t c = 0; c < G::kRegions; ++c)
+            tma_load_2d(dst + c * G::kRegion + r * 1024, v ? &tm_vr : &tm_kr, fb, c * 64, next_row + 8 * r);
+      } else if (!(next_flags & kEmpty)) {
+        mbar_arrive_expect_tx(fb, bytes + G::kHalf);
+        tma_load_2d(dst, v ? &tm_vc : &tm_kc, fb, 0, next_row);
+      } else {
+        mbar_arrive(fb);
       }
     }
     __syncwarp();
   };
-  issue(0, false);
-  issue(0, true);
 
   // ---- the worker's steps.  After a wait that ran out (the error word is
   // set) a warp waits no more, so that it still reaches the CTA's barriers.
-  uint32_t qf[H::kQShared ? 1 : kNT][kChunks][2];
   float qscale[kNT][2];  // of rows 8nt + 2t + (0, 1): the row's power of two, sm_scale and log2(e)
   float m[kNT][2], l[kNT][2];
   int limit[kNT][2];           // positions below it are seen
@@ -526,10 +553,26 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
   const int v_a = (lane >> 2) & 3, v_j = lane & 3, v_row = v_j < 2 ? 2 * v_a + v_j : 8 + ((2 * v_a + v_j - 2) ^ 4);
   const uint32_t k_off = k_row * kD + (((lane >> 4) ^ (kD == 128 ? (k_row & 7) : ((k_row >> 1) & 3))) << 4);
   const uint32_t v_off = v_row * kD + (((lane >> 4) ^ (kD == 128 ? (v_row & 7) : ((v_row >> 1) & 3))) << 4);
-  for (int k = 0; k < n_steps; ++k) {
-    const Step s = sm.step[warp][k & 1];  // written by this warp
+  Step s{};
+  s.flags = kEmpty;
+  for (int k = -1; k < n_steps; ++k) {  // (step -1 only issues the first)
+    if (k >= 0) {
+      const int from = k - batch0;
+      s.flags = next_flags;
+      s.pos0 = __shfl_sync(0xffffffffu, ahead.pos0, from);
+      s.step = __shfl_sync(0xffffffffu, ahead.step, from);
+      s.steps = __shfl_sync(0xffffffffu, ahead.steps, from);
+      s.ks = __shfl_sync(0xffffffffu, ahead.ks, from);
+      s.vs = __shfl_sync(0xffffffffu, ahead.vs, from);
+      if (s.flags & kFirst) {
+        s.b = __shfl_sync(0xffffffffu, ahead.b, from);
+        s.sub = __shfl_sync(0xffffffffu, ahead.sub, from);
+        s.len = __shfl_sync(0xffffffffu, ahead.len, from);
+        s.cnt = __shfl_sync(0xffffffffu, ahead.cnt, from);
+      }
+    }
     const bool ring = s.flags & kRingStep, empty = s.flags & kEmpty;
-    if (!aborted && !mbar_wait(smem_u32(&sm.k_full[warp]), k & 1, p.err)) aborted = true;
+    if (k >= 0 && !aborted && !mbar_wait(smem_u32(&sm.k_full[warp]), k & 1, p.err)) aborted = true;
     if (s.flags & kFirst) {
       const int h = head_of(s.sub), n0 = (s.sub - h * p.row_tiles) * kRows;
       begins = s.flags & kBegin;
@@ -549,14 +592,12 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
         // queries: fp16 fragments, k index permuted as the codes' ldmatrix gives it
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
-          uint2 raw[kChunks];  // (rows that do not exist hold anything; nothing of them is stored)
-#pragma unroll
-          for (int c = 0; c < kChunks; ++c)
-            raw[c] = *reinterpret_cast<const uint2*>(&sm.q[warp][8 * nt + g][32 * c + 8 * t]);
-          float top = 0.f;
-#pragma unroll
+          uint2* const row = reinterpret_cast<uint2*>(&sm.q[warp][8 * nt + g][8 * t]);  // (every fourth of it)
+          float top = 0.f;  // (rows that do not exist hold anything; nothing of them is stored)
+#pragma unroll 2
           for (int c = 0; c < kChunks; ++c) {
-            const float2 a = Elem<kBf16>::unpack(raw[c].x), b = Elem<kBf16>::unpack(raw[c].y);
+            const uint2 x = row[4 * c];
+            const float2 a = Elem<kBf16>::unpack(x.x), b = Elem<kBf16>::unpack(x.y);
             top = fmaxf(top, fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y))));
           }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -566,14 +607,11 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
           ex = (top == 0.f || ex == 255) ? 127 : min(max(ex, 1), 253);
           const float f = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
           const float back = __uint_as_float(static_cast<uint32_t>(ex) << 23) * p.scale_log2;
-#pragma unroll
+#pragma unroll 2
           for (int c = 0; c < kChunks; ++c) {
-            const float2 a = Elem<kBf16>::unpack(raw[c].x), b = Elem<kBf16>::unpack(raw[c].y);
-            const uint32_t lo = pack_half2(a.x * f, a.y * f), hi = pack_half2(b.x * f, b.y * f);
-            if constexpr (H::kQShared)
-              *reinterpret_cast<uint2*>(&sm.q[warp][8 * nt + g][32 * c + 8 * t]) = make_uint2(lo, hi);
-            else
-              qf[nt][c][0] = lo, qf[nt][c][1] = hi;
+            const uint2 x = row[4 * c];
+            const float2 a = Elem<kBf16>::unpack(x.x), b = Elem<kBf16>::unpack(x.y);
+            row[4 * c] = make_uint2(pack_half2(a.x * f, a.y * f), pack_half2(b.x * f, b.y * f));
           }
           qscale[nt][0] = __shfl_sync(0xffffffffu, back, 8 * t);      // from a lane of row 2t
           qscale[nt][1] = __shfl_sync(0xffffffffu, back, 8 * t + 4);  // and of 2t + 1
@@ -581,23 +619,26 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
       }
     }
     auto q_frag = [&](int nt, int c, uint32_t& b0, uint32_t& b1) {  // (a lane reads what it wrote)
-      if constexpr (H::kQShared)
-        lds8(q_at + nt * 8 * H::kQStride + 32 * c, b0, b1);
-      else
-        b0 = qf[nt][c][0], b1 = qf[nt][c][1];
+      lds8(q_at + nt * 8 * H::kQStride + 32 * c, b0, b1);
     };
     const uint32_t kb = smem_u32(sm.stage[warp]), vb = kb + G::kHalf;
-    const int n_tok = s.flags >> 8;  // of a ring step
+    const int n_tok = s.flags >> 16;  // of a ring step
     const int rounds = ring ? (n_tok + H::kTok - 1) / H::kTok : kRounds;
 
 #pragma unroll 1
     for (int round = 0; round < rounds; ++round) {
       float sc[kTC][kNT][4];
+#pragma unroll
+      for (int i = 0; i < kTC; ++i)
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][nt][e] = 0.f;
       if (!empty) {
         // ---- scores, S^T: rows g (0, 1) and g + 8 (2, 3) of 16 tokens; query rows 2t, 2t + 1
         if (!ring) {
           const uint32_t ka = kb + k_off + round * H::kTok * kD;
-#pragma unroll
+#pragma unroll kKUnroll
           for (int c = 0; c < kChunks; c += 2) {
             const uint32_t kc = ka ^ (c << 4);  // (its column is below the row's 128 or 64 bytes)
 #pragma unroll
@@ -613,46 +654,35 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
                 for (int nt = 0; nt < kNT; ++nt) {
                   uint32_t b0, b1;
                   q_frag(nt, c + j, b0, b1);
-                  if (c + j == 0)
-                    mma_first(sc[i][nt], a0, a1, a2, a3, b0, b1);
-                  else
-                    mma_16816(sc[i][nt], a0, a1, a2, a3, b0, b1);
+                  mma_16816(sc[i][nt], a0, a1, a2, a3, b0, b1);
                 }
               }
             }
           }
         } else {
+#pragma unroll kKUnroll
+          for (int c = 0; c < kChunks; ++c) {
+            uint32_t b0[kNT], b1[kNT];
 #pragma unroll
-          for (int i = 0; i < kTC; ++i)
+            for (int nt = 0; nt < kNT; ++nt) {
+              q_frag(nt, c, b0[nt], b1[nt]);
+              if constexpr (kBf16) b0[nt] = half_to_bf16(b0[nt]), b1[nt] = half_to_bf16(b1[nt]);
+            }
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) sc[i][nt][e] = 0.f;
-#pragma unroll
-          for (int i = 0; i < kRC; ++i) {
-            const int tok0 = round * H::kTok + 16 * i;
-            if (tok0 >= n_tok) break;
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c) {
-              // row & 7 == g for both of this lane's rows
-              const uint32_t at = kb + (c >> 2) * G::kRegion + (tok0 + g) * 128 +
+            for (int i = 0; i < kRC; ++i) {
+              // row & 7 == g for both of this lane's rows (those behind the tokens hold anything: masked below)
+              const uint32_t at = kb + (c >> 2) * G::kRegion + (round * H::kTok + 16 * i + g) * 128 +
                                   ((((c & 3) * 2 + (t >> 1)) ^ g) << 4) + (t & 1) * 8;
               uint32_t a0, a1, a2, a3;
               lds8(at, a0, a2);
               lds8(at + 8 * 128, a1, a3);
 #pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-                uint32_t b0, b1;
-                q_frag(nt, c, b0, b1);
-                if constexpr (kBf16) b0 = half_to_bf16(b0), b1 = half_to_bf16(b1);
-                mma_elem<kBf16>(sc[i][nt], a0, a1, a2, a3, b0, b1);
-              }
+              for (int nt = 0; nt < kNT; ++nt) mma_elem<kBf16>(sc[i][nt], a0, a1, a2, a3, b0[nt], b1[nt]);
             }
           }
         }
       }
       if (round == rounds - 1) {
-        if constexpr (H::kQShared) fence_proxy_async_smem();  // fragments stored there; a bulk copy may follow
         __syncwarp();
         issue(k + 1, false);
       }
@@ -783,9 +813,7 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
                                     ((((c & 3) * 2 + ((lane >> 3) & 1)) ^ (lane & 7)) << 4),
                                 a[0], a[1], a[2], a[3]);
               a[0] &= keep0, a[1] &= keep0, a[2] &= keep1, a[3] &= keep1;
-              const uint32_t bad = nonfinite_mask<kBf16>(a[0]) | nonfinite_mask<kBf16>(a[1]) |
-                                   nonfinite_mask<kBf16>(a[2]) | nonfinite_mask<kBf16>(a[3]);
-              if (__any_sync(0xffffffffu, bad != 0)) {
+              if (s.flags & kUnclean) {
                 // Values that are not finite would reach rows that do not see
                 // them (0 * NaN).  They are taken out, and a product of their
                 // places with the rows' masks says which sums they make NaN.
@@ -865,7 +893,7 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
     float* data = kFits && k == n_steps - 1 ? reinterpret_cast<float*>(sm.stage[warp])
                                    : p.partials + (int64_t(worker) * 2 + (begins ? 1 : 0)) * kPiece;
     if (lane == 0)
-      sm.part[warp][begins ? 1 : 0] = Part{static_cast<int>(x0) + k - s.step, data, s.b, s.sub, s.cnt, s.steps,
+      sm.part[warp][begins ? 1 : 0] = Part{x0 + k - s.step, data, s.b, s.sub, s.cnt, s.steps,
                                            kFirst | (begins ? kBegin : 0) | (s.flags & kEnd)};
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
@@ -931,16 +959,19 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
     }
   }
   if (cut[0] < 0 && cut[1] < 0) return;
-  __threadfence();
   __syncthreads();
-  auto cta_of = [&](int x) { return static_cast<int>(split.owner(x) / H::kWarps); };
+  // (borders inside a cut unit are where the split put them)
+  auto cta_of = [&](int x) { return static_cast<int>(split.owner(x)); };
   if (tid < 2) {
     sm.last[tid] = 0;
     const int c = tid ? cut[1] : cut[0];
     if (c >= 0) {
       const Part& u = sm.part[c >> 1][c & 1];
       const int c0 = cta_of(u.unit_begin), c1 = cta_of(u.unit_begin + u.steps - 1);
+      // the barrier above and this fence order the CTA's stores before its ticket
+      __threadfence();
       sm.last[tid] = atomicAdd(p.tickets + c0, 1) == c1 - c0;
+      __threadfence();
       if (sm.last[tid]) p.tickets[c0] = 0;  // ready for the next launch
     }
   }
@@ -948,7 +979,6 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     if (!sm.last[side]) continue;
-    __threadfence();
     const Part u = sm.part[cut[side] >> 1][cut[side] & 1];
     const int c0 = cta_of(u.unit_begin), c1 = cta_of(u.unit_begin + u.steps - 1);
     // the first CTA's part begins there, the others' go on from the one before
@@ -979,8 +1009,7 @@ Plan plan(const nsa_kv8_cache* c, int64_t rows) {
   const int tile = 8 * s.nt, workers = s.nt == 1 ? Shape<128, 1, true>::kWarps : Shape<128, 2, true>::kWarps;
   s.row_tiles = static_cast<int>((rows + tile - 1) / tile);
   const int64_t most = c->batch * c->n_kv_heads * s.row_tiles * (c->max_blocks + 2);  // steps
-  const int64_t ctas = (most + workers - 1) / workers;
-  s.n_ctas = static_cast<int>(ctas < max_ctas() ? ctas : max_ctas());
+  s.n_ctas = static_cast<int>(most < max_ctas() ? most : max_ctas());
   s.bytes = size_t(s.n_ctas) * (workers + 1) * 2 * tile * (2 + c->head_dim) * sizeof(float);
   return s;
 }
@@ -990,7 +1019,7 @@ int launch_attend(const Plan& plan, const CUtensorMap (&maps)[4], const AttendPa
   using S = Smem<kD, kNT, !kBf16>;
   using H = Shape<kD, kNT, !kBf16>;
   static_assert(offsetof(S, stage) == 0 && Geo<kD>::kHalf % 1024 == 0, "TMA destinations");
-  static_assert(offsetof(S, q) % 16 == 0 && offsetof(S, step) % 16 == 0, "vector reads");
+  static_assert(offsetof(S, q) % 16 == 0, "vector reads");
   static_assert(sizeof(S) <= 227 * 1024, "shared memory of an SM");
   static_assert(2 * H::kWarps <= 32, "a lane for each part");
   auto kernel = kv8_attend_kernel<kD, kNT, kBf16, kInt8>;

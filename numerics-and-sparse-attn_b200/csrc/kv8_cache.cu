@@ -31,7 +31,7 @@ int check_cache(const nsa_kv8_cache* c, Cache& out) {
   if (c->n_pages > (int64_t(1) << 31) / (c->n_kv_heads * kBlock) - 1)
     return fail(NSA_ERR_UNSUPPORTED, "n_pages * n_kv_heads * 64 must stay below 2^31");
   if (!c->k_codes || !c->v_codes || !c->scales ||
-      (c->batch > 0 && (!c->page_table || !c->k_ring || !c->v_ring || !c->lens || !c->ring_floor || !c->tickets)))
+      (c->batch > 0 && (!c->page_table || !c->k_ring || !c->v_ring || !c->lens || !c->ring_floor || !c->unclean || !c->tickets)))
     return fail(NSA_ERR_INVALID, "null pointer in the cache descriptor");
   if (!aligned16(c->k_codes) || !aligned16(c->v_codes) || !aligned16(c->k_ring) || !aligned16(c->v_ring) ||
       !aligned16(c->scales))
@@ -48,6 +48,7 @@ int check_cache(const nsa_kv8_cache* c, Cache& out) {
   out.v_ring = static_cast<uint16_t*>(c->v_ring);
   out.lens = c->lens;
   out.ring_floor = c->ring_floor;
+  out.unclean = c->unclean;
   out.tickets = c->tickets;
   return NSA_OK;
 }
@@ -236,8 +237,14 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
     for (int pos = from + row0; pos < end; pos += kRowsPass) {
       uint4 k = ldg16(nk + int64_t(pos - start) * p.k.st), v = ldg16(nv + int64_t(pos - start) * p.v.st);
       uint32_t* const w[8] = {&k.x, &k.y, &k.z, &k.w, &v.x, &v.y, &v.z, &v.w};
+      uint32_t bad = 0;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) *w[e] |= nonfinite_mask<kBf16>(*w[e]) & 0x7fff7fffu;  // NaN
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t mk = nonfinite_mask<kBf16>(*w[e]);
+        *w[e] |= mk & 0x7fff7fffu;  // NaN
+        bad |= mk;
+      }
+      if (bad) c.unclean[b] = 1;
       *reinterpret_cast<uint4*>(kr + (pos % kRing) * kD) = k;
       *reinterpret_cast<uint4*>(vr + (pos % kRing) * kD) = v;
     }

@@ -74,7 +74,7 @@ class Kv8CacheDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int64) for n in ("batch", "n_kv_heads", "head_dim", "n_pages", "max_blocks")] + \
                [(n, ctypes.c_int32) for n in ("dtype", "codes")] + \
                [(n, ctypes.c_void_p) for n in ("k_codes", "v_codes", "scales", "page_table", "k_ring", "v_ring", "lens",
-                                               "ring_floor", "tickets")]
+                                               "ring_floor", "unclean", "tickets")]
 
 
 class Kv8Rows(ctypes.Structure):
@@ -138,11 +138,11 @@ class Kv8Cache:
         if n_pages is None:
             self.page_table.copy_(torch.arange(batch * self.max_blocks, dtype=torch.int32).view(batch, -1))
         self.lens, self._ring_floor = z((batch,), torch.int64), z((batch,), torch.int64)
-        self._append_tickets = z((batch,), torch.int32)
+        self._unclean, self._append_tickets = z((batch,), torch.int32), z((batch,), torch.int32)
         d = self._desc = Kv8CacheDesc(batch, n_kv_heads, head_dim, self.n_pages, self.max_blocks, _DTYPES[dtype], code)
         for n, t in (("k_codes", self.k_codes), ("v_codes", self.v_codes), ("scales", self.scales),
                      ("page_table", self.page_table), ("k_ring", self.k_ring), ("v_ring", self.v_ring),
-                     ("lens", self.lens), ("ring_floor", self._ring_floor), ("tickets", self._append_tickets)):
+                     ("lens", self.lens), ("ring_floor", self._ring_floor), ("unclean", self._unclean), ("tickets", self._append_tickets)):
             setattr(d, n, t.data_ptr())
         self._desc_ref = ctypes.byref(d)
         self._ws_bytes = {}
