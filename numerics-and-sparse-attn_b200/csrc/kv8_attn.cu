@@ -143,7 +143,7 @@ struct Shape {
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kRows = 8 * kNT;  // of a unit
   static constexpr int kQStride = kD * 2 + 32;  // bytes: rows 8 banks apart
-  static constexpr int kTok = kNT == 4 ? 16 : 32;  // tokens of a round of scores, softmax and sums
+  static constexpr int kTok = 32;  // tokens of a round of scores, softmax and sums
 };
 
 template <int kD, int kNT, bool kSplit>
@@ -540,7 +540,6 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
   // set) a warp waits no more, so that it still reaches the CTA's barriers.
   float qscale[kNT][2];  // of rows 8nt + 2t + (0, 1): the row's power of two, sm_scale and log2(e)
   float m[kNT][2], l[kNT][2];
-  int limit[kNT][2];           // positions below it are seen
   float acc[kNT][kChunks][4];  // dims 16c + g (0, 1) and 16c + g + 8 (2, 3), rows 2t (0, 2) and 2t + 1 (1, 3)
   bool begins = false;         // the piece holds its unit's first step
   bool aborted = false;
@@ -574,15 +573,11 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
     const bool ring = s.flags & kRingStep, empty = s.flags & kEmpty;
     if (k >= 0 && !aborted && !mbar_wait(smem_u32(&sm.k_full[warp]), k & 1, p.err)) aborted = true;
     if (s.flags & kFirst) {
-      const int h = head_of(s.sub), n0 = (s.sub - h * p.row_tiles) * kRows;
       begins = s.flags & kBegin;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          m[nt][e] = -INFINITY, l[nt][e] = 0.f;
-          limit[nt][e] = limit_at(s.len, s.cnt, n0 + 8 * nt + 2 * t + e);
-        }
+        for (int e = 0; e < 2; ++e) m[nt][e] = -INFINITY, l[nt][e] = 0.f;
 #pragma unroll
         for (int c = 0; c < kChunks; ++c)
 #pragma unroll
@@ -697,14 +692,16 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
         }
         if (s.flags & kMasked) {  // (a ring step is)
           const int pos0 = s.pos0 + round * H::kTok, hi = ring ? 8 + g : 8 + (g ^ 4);
+          const int n0 = (s.sub - head_of(s.sub) * p.row_tiles) * kRows;
 #pragma unroll
-          for (int i = 0; i < kTC; ++i)
+          for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-            for (int nt = 0; nt < kNT; ++nt)
+            for (int e = 0; e < 4; ++e) {
+              const int limit = limit_at(s.len, s.cnt, n0 + 8 * nt + 2 * t + (e & 1));
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if ((ring && i >= kRC) || !sees(p, pos0 + 16 * i + (e < 2 ? g : hi), limit[nt][e & 1]))
-                  sc[i][nt][e] = -INFINITY;
+              for (int i = 0; i < kTC; ++i)
+                if ((ring && i >= kRC) || !sees(p, pos0 + 16 * i + (e < 2 ? g : hi), limit)) sc[i][nt][e] = -INFINITY;
+            }
         }
         // ---- online softmax, and P as B fragments
         float alpha[kNT][2], row_vs[kNT][2];
@@ -1005,7 +1002,7 @@ int max_ctas() {
 // Query rows of a unit: up to 8, 16 or 32; more of them are further units.
 Plan plan(const nsa_kv8_cache* c, int64_t rows) {
   Plan s;
-  s.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+  s.nt = rows <= 8 ? 1 : 2;
   const int tile = 8 * s.nt, workers = s.nt == 1 ? Shape<128, 1, true>::kWarps : Shape<128, 2, true>::kWarps;
   s.row_tiles = static_cast<int>((rows + tile - 1) / tile);
   const int64_t most = c->batch * c->n_kv_heads * s.row_tiles * (c->max_blocks + 2);  // steps
@@ -1040,8 +1037,7 @@ int launch_attend(const Plan& plan, const CUtensorMap (&maps)[4], const AttendPa
 template <int kD, bool kBf16, bool kInt8>
 int launch_rows(const Plan& s, const CUtensorMap (&maps)[4], const AttendParams& p, cudaStream_t stream) {
   if (s.nt == 1) return launch_attend<kD, 1, kBf16, kInt8>(s, maps, p, stream);
-  if (s.nt == 2) return launch_attend<kD, 2, kBf16, kInt8>(s, maps, p, stream);
-  return launch_attend<kD, 4, kBf16, kInt8>(s, maps, p, stream);
+  return launch_attend<kD, 2, kBf16, kInt8>(s, maps, p, stream);
 }
 
 int check_shape(const nsa_kv8_cache* cache, int64_t n_heads, int64_t n_tokens) {
