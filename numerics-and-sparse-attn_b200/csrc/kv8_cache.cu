@@ -138,117 +138,192 @@ __device__ __forceinline__ uint2 codes8(const uint4& x, float inv) {
 
 __device__ __forceinline__ uint4 ldg16(const uint16_t* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 
+// One thread of every CTA asks for its unit's span; the last of a sequence's
+// `askers` to have read its length sets the new one.
+__device__ __forceinline__ Span take_span(const AppendParams& p, int b, int askers) {
+  const Cache& c = p.c;
+  const int64_t len = c.lens[b], cap = int64_t(c.max_blocks) * kBlock, floor = c.ring_floor[b];
+  const int64_t s = p.starts ? p.starts[b] : len;
+  const int64_t n = p.counts ? p.counts[b] : p.n_tokens;
+  const bool ok = s >= 0 && s <= len && len <= cap && n >= 0 && n <= p.n_tokens && s + n <= cap &&
+                  (s % kBlock == 0 || s >= floor);
+  if (!ok) set_error(p.err, NSA_ERR_INVALID);
+  if (atomicAdd(c.tickets + b, 1) == askers - 1) {
+    c.tickets[b] = 0;
+    if (ok) {
+      const int64_t first = s / kBlock * kBlock, last = (s + n) / kBlock * kBlock;
+      c.lens[b] = s + n;
+      c.ring_floor[b] = max(s < floor ? first : floor, last - kBlock);
+    }
+  }
+  return Span{ok ? static_cast<int>(s) : 0, ok ? static_cast<int>(s + n) : 0, ok};
+}
+
+// Quantizes block i of a unit, which a whole CTA calls for: its tokens from
+// the ring up to `start`, from the new tokens on.
+template <int kD, bool kBf16, bool kInt8>
+__device__ __forceinline__ void quantize_block(const AppendParams& p, int b, int h, int i, int start, int tid,
+                                               float2* red) {
+  constexpr int kVecs = kD / 8;                // 16-byte vectors a row
+  constexpr int kRowsPass = kThreads / kVecs;  // rows a pass
+  constexpr int kN = kBlock / kRowsPass;       // vectors a thread of K (and of V)
+  const Cache& c = p.c;
+  const int col = (tid % kVecs) * 8, row0 = tid / kVecs;
+  const int64_t ring = (int64_t(b) * c.n_kv_heads + h) * kRing * kD + col;
+  const uint16_t* const nk = p.k.row(b, h, 0) + col;
+  const uint16_t* const nv = p.v.row(b, h, 0) + col;
+  uint4 k[kN], v[kN];
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const int pos = i * kBlock + row0 + j * kRowsPass;
+    if (pos >= start) {
+      k[j] = ldg16(nk + int64_t(pos - start) * p.k.st);
+      v[j] = ldg16(nv + int64_t(pos - start) * p.v.st);
+    } else {  // plain loads: the CTA stores to the ring afterwards
+      k[j] = *reinterpret_cast<const uint4*>(c.k_ring + ring + (pos % kRing) * kD);
+      v[j] = *reinterpret_cast<const uint4*>(c.v_ring + ring + (pos % kRing) * kD);
+    }
+  }
+  float2 m = make_float2(amax_of<kBf16, kN>(k), amax_of<kBf16, kN>(v));
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) {
+    m.x = fmaxf(m.x, __shfl_xor_sync(0xffffffffu, m.x, off));
+    m.y = fmaxf(m.y, __shfl_xor_sync(0xffffffffu, m.y, off));
+  }
+  __syncthreads();  // red is free again
+  if ((tid & 31) == 0) red[tid >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    m.x = fmaxf(m.x, red[w].x);
+    m.y = fmaxf(m.y, red[w].y);
+  }
+  constexpr float kTop = kInt8 ? 127.f : 448.f;
+  const float ks = fmaxf(__fdiv_rn(m.x, kTop), 0x1p-126f), vs = fmaxf(__fdiv_rn(m.y, kTop), 0x1p-126f);
+  const bool kbad = !(m.x < INFINITY), vbad = !(m.y < INFINITY);
+  const float ki = __frcp_rn(ks), vi = __frcp_rn(vs);
+  const int page = c.page_table[int64_t(b) * c.max_blocks + i];
+  if (page < 0 || page >= c.n_pages) {  // the block is not stored
+    if (tid == 0) set_error(p.err, NSA_ERR_INVALID);
+    return;
+  }
+  const int64_t rec = int64_t(page) * c.n_kv_heads + h;
+#pragma unroll
+  for (int j = 0; j < kN; ++j) {
+    const int64_t at = (rec * kBlock + row0 + j * kRowsPass) * kD + col;
+    const uint2 z = make_uint2(0u, 0u);
+    *reinterpret_cast<uint2*>(c.k_codes + at) = kbad ? z : codes8<kBf16, kInt8>(k[j], ki);
+    *reinterpret_cast<uint2*>(c.v_codes + at) = vbad ? z : codes8<kBf16, kInt8>(v[j], vi);
+  }
+  if (tid == 0) c.scales[rec] = make_float2(kbad ? NAN : ks, vbad ? NAN : vs);
+}
+
+// Stores a unit's tokens of its last two blocks in the ring, as they came;
+// threads `id` of `n` share the rows.
+template <int kD, bool kBf16>
+__device__ __forceinline__ void store_ring(const AppendParams& p, int b, int h, int start, int end, int id, int n) {
+  constexpr int kVecs = kD / 8;
+  const Cache& c = p.c;
+  const int col = (id % kVecs) * 8;
+  const int64_t ring = (int64_t(b) * c.n_kv_heads + h) * kRing * kD + col;
+  const uint16_t* const nk = p.k.row(b, h, 0) + col;
+  const uint16_t* const nv = p.v.row(b, h, 0) + col;
+  for (int pos = max(start, (end / kBlock - 1) * kBlock) + id / kVecs; pos < end; pos += n / kVecs) {
+    uint4 k = ldg16(nk + int64_t(pos - start) * p.k.st), v = ldg16(nv + int64_t(pos - start) * p.v.st);
+    uint32_t* const w[8] = {&k.x, &k.y, &k.z, &k.w, &v.x, &v.y, &v.z, &v.w};
+    uint32_t bad = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t mk = nonfinite_mask<kBf16>(*w[e]);
+      *w[e] |= mk & 0x7fff7fffu;  // NaN
+      bad |= mk;
+    }
+    if (bad) c.unclean[b] = 1;
+    *reinterpret_cast<uint4*>(c.k_ring + ring + (pos % kRing) * kD) = k;
+    *reinterpret_cast<uint4*>(c.v_ring + ring + (pos % kRing) * kD) = v;
+  }
+}
+
 // Grid (units, 1 + blocks that lie wholly in the new tokens).  y = 0
 // takes a unit's first block, which may begin in the ring, and then stores
 // the newest tokens there -- the same CTA, since the ring has room for two
 // blocks only and the stores can overwrite what the first block reads.
 template <int kD, bool kBf16, bool kInt8>
 __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams p) {
-  constexpr int kVecs = kD / 8;                       // 16-byte vectors a row
-  constexpr int kRowsPass = kThreads / kVecs;         // rows a pass
-  constexpr int kN = kBlock / kRowsPass;              // vectors a thread of K (and of V)
   __shared__ Span span;
   __shared__ float2 red[kThreads / 32];
   grid_launch_dependents();
   grid_dependency_wait();
   const int tid = threadIdx.x, b = blockIdx.x / p.c.n_kv_heads, h = blockIdx.x % p.c.n_kv_heads;
-  const Cache& c = p.c;
-  if (tid == 0) {
-    const int64_t len = c.lens[b], cap = int64_t(c.max_blocks) * kBlock, floor = c.ring_floor[b];
-    const int64_t s = p.starts ? p.starts[b] : len;
-    int64_t n = p.counts ? p.counts[b] : p.n_tokens;
-    const bool ok = s >= 0 && s <= len && len <= cap && n >= 0 && n <= p.n_tokens && s + n <= cap &&
-                    (s % kBlock == 0 || s >= floor);
-    if (!ok) set_error(p.err, NSA_ERR_INVALID);
-    span.ok = ok;
-    span.start = ok ? static_cast<int>(s) : 0;
-    span.end = ok ? static_cast<int>(s + n) : 0;
-    // The last CTA of the sequence to have read its length sets the new one.
-    const int arrived = atomicAdd(c.tickets + b, 1);
-    if (arrived == static_cast<int>(c.n_kv_heads * gridDim.y) - 1) {
-      c.tickets[b] = 0;
-      if (ok) {
-        const int64_t first = s / kBlock * kBlock, last = (s + n) / kBlock * kBlock;
-        c.lens[b] = s + n;
-        c.ring_floor[b] = max(s < floor ? first : floor, last - kBlock);
-      }
-    }
-  }
+  if (tid == 0) span = take_span(p, b, p.c.n_kv_heads * gridDim.y);
   __syncthreads();
   if (!span.ok) return;
-  const int start = span.start, end = span.end, first = start / kBlock, done = end / kBlock;
-  const int col = (tid % kVecs) * 8, row0 = tid / kVecs;
-  const int64_t unit = blockIdx.x;
-  uint16_t* const kr = c.k_ring + unit * kRing * kD + col;
-  uint16_t* const vr = c.v_ring + unit * kRing * kD + col;
-  const uint16_t* const nk = p.k.row(b, h, 0) + col;
-  const uint16_t* const nv = p.v.row(b, h, 0) + col;
+  const int start = span.start, end = span.end;
+  for (int i = start / kBlock + blockIdx.y; i < end / kBlock; i += gridDim.y)
+    quantize_block<kD, kBf16, kInt8>(p, b, h, i, start, tid, red);
+  if (blockIdx.y == 0) {
+    __syncthreads();  // every thread has read what it needs of the ring
+    store_ring<kD, kBf16>(p, b, h, start, end, tid, kThreads);
+  }
+}
 
-  for (int i = first + blockIdx.y; i < done; i += gridDim.y) {
-    uint4 k[kN], v[kN];
-#pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      const int pos = i * kBlock + row0 + j * kRowsPass;
-      if (pos >= start) {
-        k[j] = ldg16(nk + int64_t(pos - start) * p.k.st);
-        v[j] = ldg16(nv + int64_t(pos - start) * p.v.st);
-      } else {  // plain loads: this CTA stores to the ring below
-        k[j] = *reinterpret_cast<const uint4*>(kr + (pos % kRing) * kD);
-        v[j] = *reinterpret_cast<const uint4*>(vr + (pos % kRing) * kD);
-      }
-    }
-    float2 m = make_float2(amax_of<kBf16, kN>(k), amax_of<kBf16, kN>(v));
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) {
-      m.x = fmaxf(m.x, __shfl_xor_sync(0xffffffffu, m.x, off));
-      m.y = fmaxf(m.y, __shfl_xor_sync(0xffffffffu, m.y, off));
-    }
-    __syncthreads();  // red is free again
-    if ((tid & 31) == 0) red[tid >> 5] = m;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      m.x = fmaxf(m.x, red[w].x);
-      m.y = fmaxf(m.y, red[w].y);
-    }
-    constexpr float kTop = kInt8 ? 127.f : 448.f;
-    const float ks = fmaxf(__fdiv_rn(m.x, kTop), 0x1p-126f), vs = fmaxf(__fdiv_rn(m.y, kTop), 0x1p-126f);
-    const bool kbad = !(m.x < INFINITY), vbad = !(m.y < INFINITY);
-    const float ki = __frcp_rn(ks), vi = __frcp_rn(vs);
+// The same for fewer new tokens than a block has, a smaller CTA a unit: most
+// units only store a row or a few, so what counts is how many CTAs are resident
+// at once; K and V of a block that is completed take turns in the registers.
+constexpr int kFewThreads = 256;
+template <int kD, bool kBf16, bool kInt8>
+__global__ void __launch_bounds__(kFewThreads) kv8_append_few_kernel(const AppendParams p) {
+  constexpr int kVecs = kD / 8, kRowsPass = kFewThreads / kVecs, kN = kBlock / kRowsPass;
+  constexpr float kTop = kInt8 ? 127.f : 448.f;
+  __shared__ Span span;
+  __shared__ float red[2][kFewThreads / 32];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const Cache& c = p.c;
+  const int tid = threadIdx.x, b = blockIdx.x / c.n_kv_heads, h = blockIdx.x % c.n_kv_heads;
+  if (tid == 0) span = take_span(p, b, c.n_kv_heads);
+  __syncthreads();
+  if (!span.ok) return;
+  const int start = span.start, end = span.end, i = start / kBlock;
+  if (end / kBlock != i) {  // block i is completed
     const int page = c.page_table[int64_t(b) * c.max_blocks + i];
-    if (page < 0 || page >= c.n_pages) {  // the block is not stored
+    if (page < 0 || page >= c.n_pages) {  // it is not stored
       if (tid == 0) set_error(p.err, NSA_ERR_INVALID);
-      continue;
-    }
-    const int64_t rec = int64_t(page) * c.n_kv_heads + h;
+    } else {
+      const int64_t rec = int64_t(page) * c.n_kv_heads + h;
+      const int col = (tid % kVecs) * 8, row0 = tid / kVecs;
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t) {
+        const uint16_t* const ring = (t ? c.v_ring : c.k_ring) + int64_t(blockIdx.x) * kRing * kD + col;
+        const Rows& rows = t ? p.v : p.k;
+        const uint16_t* const fresh = rows.row(b, h, 0) + col;
+        uint8_t* const codes = (t ? c.v_codes : c.k_codes) + rec * kBlock * kD + col;
+        uint4 x[kN];
 #pragma unroll
-    for (int j = 0; j < kN; ++j) {
-      const int64_t at = (rec * kBlock + row0 + j * kRowsPass) * kD + col;
-      const uint2 z = make_uint2(0u, 0u);
-      *reinterpret_cast<uint2*>(c.k_codes + at) = kbad ? z : codes8<kBf16, kInt8>(k[j], ki);
-      *reinterpret_cast<uint2*>(c.v_codes + at) = vbad ? z : codes8<kBf16, kInt8>(v[j], vi);
-    }
-    if (tid == 0) c.scales[rec] = make_float2(kbad ? NAN : ks, vbad ? NAN : vs);
-  }
-
-  if (blockIdx.y == 0) {  // the tokens of the last two blocks, as they came
-    __syncthreads();      // every thread has read what it needs of the ring
-    const int from = max(start, (done - 1) * kBlock);
-    for (int pos = from + row0; pos < end; pos += kRowsPass) {
-      uint4 k = ldg16(nk + int64_t(pos - start) * p.k.st), v = ldg16(nv + int64_t(pos - start) * p.v.st);
-      uint32_t* const w[8] = {&k.x, &k.y, &k.z, &k.w, &v.x, &v.y, &v.z, &v.w};
-      uint32_t bad = 0;
+        for (int j = 0; j < kN; ++j) {
+          const int pos = i * kBlock + row0 + j * kRowsPass;
+          x[j] = *reinterpret_cast<const uint4*>(pos >= start ? fresh + int64_t(pos - start) * rows.st
+                                                              : ring + (pos % kRing) * kD);
+        }
+        float m = amax_of<kBf16, kN>(x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const uint32_t mk = nonfinite_mask<kBf16>(*w[e]);
-        *w[e] |= mk & 0x7fff7fffu;  // NaN
-        bad |= mk;
+        for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+        if ((tid & 31) == 0) red[t][tid >> 5] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kFewThreads / 32; ++w) m = fmaxf(m, red[t][w]);
+        const bool bad = !(m < INFINITY);
+        const float scale = fmaxf(__fdiv_rn(m, kTop), 0x1p-126f), inv = __frcp_rn(scale);
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+          *reinterpret_cast<uint2*>(codes + (row0 + j * kRowsPass) * kD) =
+              bad ? make_uint2(0u, 0u) : codes8<kBf16, kInt8>(x[j], inv);
+        if (tid == 0) reinterpret_cast<float*>(c.scales + rec)[t] = bad ? NAN : scale;
       }
-      if (bad) c.unclean[b] = 1;
-      *reinterpret_cast<uint4*>(kr + (pos % kRing) * kD) = k;
-      *reinterpret_cast<uint4*>(vr + (pos % kRing) * kD) = v;
     }
   }
+  __syncthreads();  // every thread has read what it needs of the ring
+  store_ring<kD, kBf16>(p, b, h, start, end, tid, kFewThreads);
 }
 
 // ---------------------------------------------------------------- read back
@@ -374,7 +449,14 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const ReadParams p) 
 }
 
 template <int kD, bool kBf16, bool kInt8>
-cudaError_t launch_append(const AppendParams& p, dim3 grid, cudaStream_t stream) {
+cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
+  const int64_t units = int64_t(p.c.batch) * p.c.n_kv_heads;
+  if (p.n_tokens < kBlock) {  // at most one block is completed
+    return launch_kernel(kv8_append_few_kernel<kD, kBf16, kInt8>, dim3(static_cast<unsigned>(units)), dim3(kFewThreads),
+                         0, stream, p);
+  }
+  const int more = (p.n_tokens + kBlock - 1) / kBlock;  // blocks besides a unit's first
+  const dim3 grid(static_cast<unsigned>(units), 1 + static_cast<unsigned>(more < 65534 ? more : 65534));
   return launch_kernel(kv8_append_kernel<kD, kBf16, kInt8>, grid, dim3(kThreads), 0, stream, p);
 }
 template <int kD, bool kBf16, bool kInt8>
@@ -419,11 +501,7 @@ extern "C" int nsa_kv8_append(const nsa_kv8_cache* cache, const nsa_kv8_rows* ne
   p.counts = counts;
   p.err = device_error_word();
   if (!p.err) return fail(NSA_ERR_CUDA, "device error word unavailable");
-  // blocks that n_tokens can complete besides a unit's first
-  const int64_t more = (n_tokens + kv8::kBlock - 1) / kv8::kBlock;
-  const int64_t y = 1 + (n_tokens >= kv8::kBlock ? (more < 65534 ? more : 65534) : 0);
-  const dim3 grid(static_cast<unsigned>(p.c.batch) * p.c.n_kv_heads, static_cast<unsigned>(y));
-  cudaError_t e = NSA_KV8_DISPATCH(cache, kv8::launch_append, p, grid, stream);
+  cudaError_t e = NSA_KV8_DISPATCH(cache, kv8::launch_append, p, stream);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? NSA_OK : cuda_fail(e, "kv8_append_kernel launch");
 }

@@ -83,11 +83,30 @@ class Kv8Rows(ctypes.Structure):
                                                                            "token_stride")]
 
 
-def _rows(t):
-    """[B, H, D] or [B, H, T, D] as nsa_kv8_rows; dimensions of one element have no stride."""
-    shape, st = t.shape, t.stride()
-    return ctypes.byref(Kv8Rows(t.data_ptr(), st[0] if shape[0] > 1 else 0, st[1] if shape[1] > 1 else 0,
-                                st[2] if len(shape) == 4 and shape[2] > 1 else 0))
+class _RowArgs(threading.local):
+    """nsa_kv8_rows of a call's tensors, one set a thread (making them anew costs 2 us each)."""
+
+    def __init__(self):
+        self.rows = [Kv8Rows() for _ in range(4)]
+        self.refs = [ctypes.byref(r) for r in self.rows]
+
+
+_row_args = _RowArgs()
+
+
+def _rows(i, t, args=_row_args):
+    """[B, H, D] or [B, H, T, D] as the call's i-th nsa_kv8_rows; dimensions of one element have no stride."""
+    row, shape, st = args.rows[i], t.shape, t.stride()
+    row.data = t.data_ptr()
+    row.batch_stride = st[0] if shape[0] > 1 else 0
+    row.head_stride = st[1] if shape[1] > 1 else 0
+    row.token_stride = st[2] if len(shape) == 4 and shape[2] > 1 else 0
+    return args.refs[i]
+
+
+def _stream(index):
+    """Raw handle of the device's current stream (a Stream object costs 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class Kv8Cache:
@@ -145,46 +164,65 @@ class Kv8Cache:
                      ("lens", self.lens), ("ring_floor", self._ring_floor), ("unclean", self._unclean), ("tickets", self._append_tickets)):
             setattr(d, n, t.data_ptr())
         self._desc_ref = ctypes.byref(d)
-        self._ws_bytes = {}
+        self._lib, self._index, self._ws_bytes = _lib.load(), device.index, {}
         _graph_rows(device)
 
     # ---------------------------------------------------------------- plumbing
+    # (messages are built where they are raised: these checks run on every call)
     def _check(self, name, t, heads):
-        """Checks [B, heads, D] or [B, heads, T, D]; returns T."""
-        _req(isinstance(t, torch.Tensor), f"{name} must be a torch.Tensor", TypeError)
-        _req(t.device == self.device, f"{name} must be a CUDA tensor on the cache's device {self.device} (no CPU fallback)")
-        _req(t.dtype == self.dtype, f"{name} must be {self.dtype}, got {t.dtype}", TypeError)
+        """Checks [B, heads, D] or [B, heads, T, D] (heads 0: any multiple of the KV heads); returns T."""
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.get_device() != self._index:
+            raise ValueError(f"{name} must be a CUDA tensor on the cache's device {self.device} (no CPU fallback)")
+        if t.dtype != self.dtype:
+            raise TypeError(f"{name} must be {self.dtype}, got {t.dtype}")
         shape = t.shape
-        _req(len(shape) in (3, 4) and shape[0] == self.batch and shape[-1] == self.head_dim
-             and (shape[1] == heads if heads else shape[1] > 0 and shape[1] % self.n_kv_heads == 0),
-             f"{name} must be [{self.batch}, {heads or f'multiple of {self.n_kv_heads}'}, (T,) {self.head_dim}], "
-             f"got {tuple(shape)}")
-        _req(t.stride(-1) == 1, f"the last dimension of {name} must be contiguous")
-        return shape[2] if len(shape) == 4 else 1
+        n = len(shape)
+        if not ((n == 3 or n == 4) and shape[0] == self.batch and shape[-1] == self.head_dim
+                and (shape[1] == heads if heads else shape[1] > 0 and shape[1] % self.n_kv_heads == 0)):
+            raise ValueError(f"{name} must be [{self.batch}, {heads or f'multiple of {self.n_kv_heads}'}, (T,) "
+                             f"{self.head_dim}], got {tuple(shape)}")
+        if t.stride(-1) != 1:
+            raise ValueError(f"the last dimension of {name} must be contiguous")
+        return shape[2] if n == 4 else 1
 
     def _words(self, name, t):
         """Device pointer of an optional int64 [B] tensor."""
         if t is None:
             return None
-        _req(isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.device == self.device
-             and t.shape == (self.batch,) and t.is_contiguous(),
-             f"{name} must be a contiguous int64 CUDA tensor of length B on the cache's device")
+        if not (isinstance(t, torch.Tensor) and t.dtype == torch.int64 and t.get_device() == self._index
+                and t.shape == (self.batch,) and t.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous int64 CUDA tensor of length B on the cache's device")
         return t.data_ptr()
 
-    def _scratch(self, heads, n_tokens, stream):
+    def _call(self, fn, *args):
+        """fn(descriptor, *args, current stream of the cache's device), its status checked."""
+        if torch._C._cuda_getDevice() == self._index:
+            status = fn(self._desc_ref, *args, _stream(self._index))
+        else:
+            with torch.cuda.device(self._index):
+                status = fn(self._desc_ref, *args, _stream(self._index))
+        if status:
+            _lib.check(status)
+
+    def _scratch(self, heads, n_tokens):
         """Workspace and tickets of one attend."""
         nbytes = self._ws_bytes.get((heads, n_tokens))
         if nbytes is None:
-            nbytes = _lib.load().nsa_kv8_workspace_bytes(self._desc_ref, heads, n_tokens)
+            nbytes = self._lib.nsa_kv8_workspace_bytes(self._desc_ref, heads, n_tokens)
             if self.batch and not nbytes:
                 _lib.check(_lib.NSA_ERR_INVALID)  # raises with the library's message
             self._ws_bytes[heads, n_tokens] = nbytes
-        return _scratch(self.device, nbytes, stream)
+        return _scratch(self.device, nbytes, _stream(self._index))
 
-    def _mask(self, window, sink):
+    def _attend_args(self, sm_scale, window, sink):
+        if window is not None and window < 0:
+            raise ValueError("window must not be negative")
         window, sink = -1 if window is None else int(window), int(sink)
-        _req(window >= -1 and sink >= 0, "window and sink must not be negative")
-        return window, sink
+        if sink < 0:
+            raise ValueError("sink must not be negative")
+        return window, sink, self.head_dim ** -0.5 if sm_scale is None else float(sm_scale)
 
     # ---------------------------------------------------------------- writing
     def append(self, new_k, new_v, counts=None, starts=None):
@@ -196,19 +234,15 @@ class Kv8Cache:
         back (any multiple of 64, or as far as the block before the one in
         which the last append ended)."""
         t = self._check("new_k", new_k, self.n_kv_heads)
-        _req(self._check("new_v", new_v, self.n_kv_heads) == t and new_v.dim() == new_k.dim(),
-             "new_k and new_v must have the same shape")
-        with _lib.on_device(self.device):
-            _lib.check(_lib.load().nsa_kv8_append(self._desc_ref, _rows(new_k), _rows(new_v), t,
-                                                  self._words("starts", starts), self._words("counts", counts),
-                                                  _lib.stream_handle(self.device)))
+        if self._check("new_v", new_v, self.n_kv_heads) != t or new_v.dim() != new_k.dim():
+            raise ValueError("new_k and new_v must have the same shape")
+        self._call(self._lib.nsa_kv8_append, _rows(0, new_k), _rows(1, new_v), t, self._words("starts", starts),
+                   self._words("counts", counts))
 
     def truncate(self, lens):
         """Set the lengths to ``lens`` (int64 [B]), taking tokens back as
         ``append``'s ``starts`` does (0 empties a sequence)."""
-        with _lib.on_device(self.device):
-            _lib.check(_lib.load().nsa_kv8_append(self._desc_ref, None, None, 0, self._words("lens", lens), None,
-                                                  _lib.stream_handle(self.device)))
+        self._call(self._lib.nsa_kv8_append, None, None, 0, self._words("lens", lens), None)
 
     # ---------------------------------------------------------------- reading
     def read(self, n_tokens, starts=None, dtype=None):
@@ -221,9 +255,8 @@ class Kv8Cache:
         _req(n_tokens >= 0, "n_tokens must not be negative")
         k, v = (torch.empty((self.batch, self.n_kv_heads, n_tokens, self.head_dim), dtype=dtype, device=self.device)
                 for _ in range(2))
-        with _lib.on_device(self.device):
-            _lib.check(_lib.load().nsa_kv8_read(self._desc_ref, n_tokens, self._words("starts", starts), k.data_ptr(),
-                                                v.data_ptr(), _DTYPES[dtype], _lib.stream_handle(self.device)))
+        self._call(self._lib.nsa_kv8_read, n_tokens, self._words("starts", starts), k.data_ptr(), v.data_ptr(),
+                   _DTYPES[dtype])
         return k, v
 
     # ---------------------------------------------------------------- attention
@@ -236,35 +269,25 @@ class Kv8Cache:
         first ``sink``.  ``counts`` (int64 [B]): how many of the T query tokens
         each sequence has (row i then at lens - counts + i).  Rows that see
         nothing and rows behind counts are 0."""
-        t = self._check("q", q, 0)
-        heads = q.shape[1]
-        window, sink = self._mask(window, sink)
+        t, heads = self._check("q", q, 0), q.shape[1]
+        window, sink, scale = self._attend_args(sm_scale, window, sink)
         o = torch.empty_like(q)
-        with _lib.on_device(self.device):
-            stream = _lib.stream_handle(self.device)
-            ws, tickets = self._scratch(heads, t, stream)
-            _lib.check(_lib.load().nsa_kv8_attend(
-                self._desc_ref, _rows(q), _rows(o), heads, t, self._words("counts", counts), window, sink,
-                self.head_dim ** -0.5 if sm_scale is None else float(sm_scale), ws.data_ptr(), ws.numel(),
-                tickets.data_ptr(), stream))
+        ws, tickets = self._scratch(heads, t)
+        self._call(self._lib.nsa_kv8_attend, _rows(0, q), _rows(1, o), heads, t, self._words("counts", counts), window,
+                   sink, scale, ws.data_ptr(), ws.numel(), tickets.data_ptr())
         return o
 
     def decode_step(self, q, new_k, new_v, sm_scale=None, window=None, sink=SINK_SIZE, counts=None, starts=None):
         """append(new_k, new_v, counts, starts), then attend(q, ...) with the
         new tokens as queries: q [B, H, D] with new_k / new_v [B, Hkv, D], or
         all three with T tokens."""
-        t = self._check("q", q, 0)
-        _req(self._check("new_k", new_k, self.n_kv_heads) == t and self._check("new_v", new_v, self.n_kv_heads) == t,
-             "q, new_k and new_v must hold the same number of tokens")
-        heads = q.shape[1]
-        window, sink = self._mask(window, sink)
+        t, heads = self._check("q", q, 0), q.shape[1]
+        if self._check("new_k", new_k, self.n_kv_heads) != t or self._check("new_v", new_v, self.n_kv_heads) != t:
+            raise ValueError("q, new_k and new_v must hold the same number of tokens")
+        window, sink, scale = self._attend_args(sm_scale, window, sink)
         o = torch.empty_like(q)
-        with _lib.on_device(self.device):
-            stream = _lib.stream_handle(self.device)
-            ws, tickets = self._scratch(heads, t, stream)
-            _lib.check(_lib.load().nsa_kv8_decode_step(
-                self._desc_ref, _rows(new_k), _rows(new_v), _rows(q), _rows(o), heads, t,
-                self._words("starts", starts), self._words("counts", counts), window, sink,
-                self.head_dim ** -0.5 if sm_scale is None else float(sm_scale), ws.data_ptr(), ws.numel(),
-                tickets.data_ptr(), stream))
+        ws, tickets = self._scratch(heads, t)
+        self._call(self._lib.nsa_kv8_decode_step, _rows(0, new_k), _rows(1, new_v), _rows(2, q), _rows(3, o), heads, t,
+                   self._words("starts", starts), self._words("counts", counts), window, sink, scale, ws.data_ptr(),
+                   ws.numel(), tickets.data_ptr())
         return o
