@@ -155,7 +155,7 @@ class Kv8Cache:
         self.k_ring, self.v_ring = z(ring, dtype), z(ring, dtype)
         self.page_table = z((batch, self.max_blocks), torch.int32)
         if n_pages is None:
-            self.page_table.copy_(torch.arange(batch * self.max_blocks, dtype=torch.int32).view(batch, -1))
+            self.page_table.copy_(torch.arange(batch * self.max_blocks, dtype=torch.int32).view(batch, self.max_blocks))
         self.lens, self._ring_floor = z((batch,), torch.int64), z((batch,), torch.int64)
         self._unclean, self._append_tickets = z((batch,), torch.int32), z((batch,), torch.int32)
         d = self._desc = Kv8CacheDesc(batch, n_kv_heads, head_dim, self.n_pages, self.max_blocks, _DTYPES[dtype], code)
