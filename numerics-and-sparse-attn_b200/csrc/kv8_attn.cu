@@ -34,7 +34,7 @@ namespace kv8 {
 namespace {
 
 constexpr int kShare = 6;   // steps of a CTA at least, where there are more CTAs than units
-constexpr int kWhole = 32;  // steps of a unit that is not cut between CTAs
+constexpr int kMerge = 16;  // steps that take a CTA as long as a merge across CTAs
 constexpr int kLensCached = 512;  // sequence lengths kept in shared memory
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -153,7 +153,7 @@ struct Smem {
   uint8_t q[H::kWarps][H::kRows][H::kQStride];
   Part part[H::kWarps][2];
   int2 lens[kLensCached];
-  int scan[H::kWarps];
+  int2 scan[H::kWarps];  // steps and the longest unit of each warp's sequences
   int before[H::kThreads];  // steps before a thread's sequences
   int range[2];  // the CTA's steps
   int last[2];  // whether this CTA was the last of its first / last cut unit
@@ -350,11 +350,13 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
   // ---- the split: steps before each thread's run of sequences
   const int batch = p.c.batch, per = (batch + H::kThreads - 1) / H::kThreads;
   const int units = p.c.n_kv_heads * p.row_tiles;  // of a sequence
-  int mine = 0;  // steps of this thread's sequences, of one unit
+  int mine = 0, longest = 0;  // steps of this thread's sequences, of one unit
   for (int b = tid * per; b < min(batch, (tid + 1) * per); ++b) {
     const int2 l = load_len(p, b);
     if (b < kLensCached) sm.lens[b] = l;
-    mine += make_seq(p, l.x, l.y).steps;
+    const int steps = make_seq(p, l.x, l.y).steps;
+    mine += steps;
+    longest = max(longest, steps);
   }
   int before = mine;
 #pragma unroll
@@ -362,13 +364,15 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
     const int y = __shfl_up_sync(0xffffffffu, before, off);
     if (lane >= off) before += y;
   }
-  if (lane == 31) sm.scan[warp] = before;
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 31) sm.scan[warp] = make_int2(before, longest);
   __syncthreads();
   int sum = 0, prior = 0;
 #pragma unroll
   for (int i = 0; i < H::kWarps; ++i) {
     if (i == warp) prior = sum;
-    sum += sm.scan[i];
+    sum += sm.scan[i].x;
+    longest = max(longest, sm.scan[i].y);
   }
   if (int64_t(sum) * units > 0x7fffffff) {  // (16 TB of codes)
     if (tid == 0) set_error(p.err, NSA_ERR_INVALID);
@@ -401,15 +405,21 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
   const uint32_t total = static_cast<uint32_t>(sum) * units;
   const Split split(total, min(gridDim.x, max((total + kShare - 1) / kShare, static_cast<uint32_t>(batch * units))));
   if (blockIdx.x >= split.n) return;
-  // A CTA's range ends at unit borders where the unit there is short: a merge
-  // across CTAs costs as much as about kWhole steps of a CTA.
+  // A CTA's range ends at a unit's border where that costs less than a merge
+  // across CTAs, about kMerge steps of a CTA's time: where the unit there has at
+  // most twice as many (a border moves by half of it at most), and everywhere
+  // where the CTA with most units has few steps above the average.  (B = 16, L =
+  // 4096, 8 KV heads: 37.5 us with cut units, 31 with whole ones; B = 1: 18 and 26.)
+  const int n_units = batch * units;
+  const int whole = (n_units + static_cast<int>(split.n) - 1) / static_cast<int>(split.n) * longest <=
+                            static_cast<int>(split.each) + kMerge ? longest : 2 * kMerge;
   if (warp < 2) {
     const uint32_t c = blockIdx.x + warp;
     int x = split.begin(c);
     if (x > 0 && c < split.n) {
       const Found f = find(x);
       const int in = (x - f.begin) % f.steps;
-      if (f.steps <= kWhole) x += 2 * in < f.steps ? -in : f.steps - in;
+      if (f.steps <= whole) x += 2 * in < f.steps ? -in : f.steps - in;
     }
     if (lane == 0) sm.range[warp] = x;
   }

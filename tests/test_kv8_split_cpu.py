@@ -6,7 +6,7 @@ import random
 
 import pytest
 
-WHOLE = 32  # units of at most this many steps are not cut between CTAs
+MERGE = 16  # steps that take a CTA as long as a merge across CTAs
 
 
 class Split:
@@ -34,23 +34,30 @@ def _unit_at(steps, units, x):
     raise AssertionError(x)
 
 
+def _whole(split, steps, units):
+    """Units of at most this many steps are not cut between CTAs."""
+    most = -(-len(steps) * units // split.n) * max(steps)
+    return max(steps) if most <= split.each + MERGE else 2 * MERGE
+
+
 def _border(split, steps, units, c):
     x = split.begin(c)
     if 0 < x and c < split.n:
         b, _, inside, _ = _unit_at(steps, units, x)
-        if steps[b] <= WHOLE:
+        if steps[b] <= _whole(split, steps, units):
             x += -inside if 2 * inside < steps[b] else steps[b] - inside
     return x
 
 
 @pytest.mark.parametrize("warps", [8, 12])
-@pytest.mark.parametrize("seed", range(12))
+@pytest.mark.parametrize("seed", range(18))
 def test_every_step_is_taken_once_and_parts_join(seed, warps):
     rng = random.Random(seed)
     ctas = rng.choice([1, 3, 16, 37])
     units = rng.choice([1, 2, 8])
     longest = rng.choice([1, 6, 33, 90, 400])
-    steps = [rng.randint(1, longest) for _ in range(rng.choice([1, 2, 9, 40]))]
+    even = seed % 3 == 0
+    steps = [longest if even else rng.randint(1, longest) for _ in range(rng.choice([1, 2, 9, 40]))]
     total = sum(steps) * units
     split = Split(total, ctas)
     taken = []
@@ -95,6 +102,6 @@ def test_every_step_is_taken_once_and_parts_join(seed, warps):
     assert taken == list(range(total))
     for first, where in parts_of.items():
         b = _unit_at(steps, units, first)[0]
-        assert steps[b] > WHOLE
+        assert steps[b] > _whole(split, steps, units)
         c0, c1 = split.owner(first), split.owner(first + steps[b] - 1)
         assert where == [(c, int(c == c0)) for c in range(c0, c1 + 1)]  # what the last of them merges
