@@ -133,13 +133,12 @@ struct Part {
   int flags;  // 0: none; else kFirst and whether it holds the unit's begin / end
 };
 
-// One CTA per SM.  12 warps of 168 registers where 8 query rows leave room for
-// them, else 8 of 255; the shared memory left over goes to their stages.  With 32
-// rows the query fragments are read from shared memory (64 registers of 128
-// dimensions otherwise).
+// One CTA per SM.  12 warps of 168 registers where the accumulators leave room
+// (up to 8 query rows of 128 dimensions, 16 of 64), else 8 of 255.  Spilled
+// registers are dear here: with this much shared memory they miss the L1.
 template <int kD, int kNT, bool kSplit>
 struct Shape {
-  static constexpr int kWarps = kNT == 1 ? 12 : 8;
+  static constexpr int kWarps = kNT * kD <= 128 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
   static constexpr int kRows = 8 * kNT;  // of a unit
   static constexpr int kQStride = kD * 2 + 32;  // bytes: rows 8 banks apart
@@ -1013,7 +1012,8 @@ int max_ctas() {
 Plan plan(const nsa_kv8_cache* c, int64_t rows) {
   Plan s;
   s.nt = rows <= 8 ? 1 : 2;
-  const int tile = 8 * s.nt, workers = s.nt == 1 ? Shape<128, 1, true>::kWarps : Shape<128, 2, true>::kWarps;
+  const int tile = 8 * s.nt;
+  const int workers = s.nt * c->head_dim <= 128 ? Shape<128, 1, true>::kWarps : Shape<128, 2, true>::kWarps;
   s.row_tiles = static_cast<int>((rows + tile - 1) / tile);
   const int64_t most = c->batch * c->n_kv_heads * s.row_tiles * (c->max_blocks + 2);  // steps
   s.n_ctas = static_cast<int>(most < max_ctas() ? most : max_ctas());
