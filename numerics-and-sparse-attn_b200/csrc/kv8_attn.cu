@@ -43,6 +43,7 @@ struct AttendParams {
   Rows q, o;
   int group, n_tokens, rows, row_tiles;  // rows = n_tokens * group of a KV head
   uint32_t group_inv;                    // ceil(2^32 / group)
+  float units_inv;                       // 1 / (KV heads * row_tiles)
   const int64_t* counts;
   int window, sink;  // window < 0: all positions
   float scale_log2;
@@ -154,7 +155,6 @@ struct Smem {
   int2 lens[kLensCached];
   int2 scan[H::kWarps];  // steps and the longest unit of each warp's sequences
   int before[H::kThreads];  // steps before a thread's sequences
-  int range[2];  // the CTA's steps
   int last[2];  // whether this CTA was the last of its first / last cut unit
   uint64_t k_full[H::kWarps], v_full[H::kWarps];
 };
@@ -366,40 +366,16 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
   longest = __reduce_max_sync(0xffffffffu, longest);
   if (lane == 31) sm.scan[warp] = make_int2(before, longest);
   __syncthreads();
-  int sum = 0, prior = 0;
-#pragma unroll
-  for (int i = 0; i < H::kWarps; ++i) {
-    if (i == warp) prior = sum;
-    sum += sm.scan[i].x;
-    longest = max(longest, sm.scan[i].y);
-  }
-  if (int64_t(sum) * units > 0x7fffffff) {  // (16 TB of codes)
+  const int2 of_warp = lane < H::kWarps ? sm.scan[lane] : make_int2(0, 0);
+  const int sum = __reduce_add_sync(0xffffffffu, of_warp.x);
+  const int prior = __reduce_add_sync(0xffffffffu, lane < warp ? of_warp.x : 0);
+  longest = __reduce_max_sync(0xffffffffu, of_warp.y);
+  if (__umulhi(sum, units) != 0 || static_cast<int>(static_cast<uint32_t>(sum) * units) < 0) {  // (16 TB of codes)
     if (tid == 0) set_error(p.err, NSA_ERR_INVALID);
     return;
   }
   sm.before[tid] = before + prior - mine;
   __syncthreads();
-  // The sequence that holds step x: the last one that begins at it or before.
-  const int threads = (batch + per - 1) / per;
-  struct Found {
-    int b, begin, steps;  // the sequence's first step, and its steps a unit
-  };
-  auto find = [&](int x) {  // (a whole warp)
-    const int at = x / units;
-    int n = 0;
-    for (int i = lane; i < threads; i += 32) n += sm.before[i] <= at;
-    n = __reduce_add_sync(0xffffffffu, n) - 1;
-    Found f{n * per, sm.before[n], 0};
-    for (;;) {
-      const int2 l = f.b < kLensCached ? sm.lens[f.b] : load_len(p, f.b);
-      f.steps = make_seq(p, l.x, l.y).steps;
-      if (at < f.begin + f.steps) break;
-      f.begin += f.steps;
-      ++f.b;
-    }
-    f.begin *= units;
-    return f;
-  };
   // a CTA for every kShare steps, or for every unit
   const uint32_t total = static_cast<uint32_t>(sum) * units;
   const Split split(total, min(gridDim.x, max((total + kShare - 1) / kShare, static_cast<uint32_t>(batch * units))));
@@ -409,36 +385,65 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
   // most twice as many (a border moves by half of it at most), and everywhere
   // where the CTA with most units has few steps above the average.  (B = 16, L =
   // 4096, 8 KV heads: 37.5 us with cut units, 31 with whole ones; B = 1: 18 and 26.)
-  const int n_units = batch * units;
-  const int whole = (n_units + static_cast<int>(split.n) - 1) / static_cast<int>(split.n) * longest <=
-                            static_cast<int>(split.each) + kMerge ? longest : 2 * kMerge;
-  if (warp < 2) {
-    const uint32_t c = blockIdx.x + warp;
-    int x = split.begin(c);
-    if (x > 0 && c < split.n) {
-      const Found f = find(x);
-      const int in = (x - f.begin) % f.steps;
-      if (f.steps <= whole) x += 2 * in < f.steps ? -in : f.steps - in;
+  // (a quotient one too low or high only shifts that choice, the same for all)
+  const int whole_each = static_cast<int>(__fdividef(static_cast<float>(split.each + kMerge), static_cast<float>(longest)));
+  const int whole = batch * units <= static_cast<int>(split.n) * whole_each ? longest : 2 * kMerge;
+  // Which sequence holds step x?  Asked for the CTA's two borders, by the halves
+  // of every warp, and again for the warp's own first step where that is not in
+  // the first border's sequence.
+  int x = split.begin(blockIdx.x + (lane >> 4));
+  const int threads = (batch + per - 1) / per;
+  int cur_b = 0, cur_rel = 0;  // a sequence, and its first step from the worker's first
+  int x0 = 0, n_steps = 0;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const int ask = pass == 0 && x == static_cast<int>(total) ? 0 : x;
+    // ask / units: a quotient in float32, what it left over divided again, and one step at most to go
+    int at = __float2int_rz(__int2float_rz(ask) * p.units_inv);
+    at += __float2int_rn(__int2float_rn(ask - at * units) * p.units_inv);
+    at -= at * units > ask;
+    at += (at + 1) * units <= ask;
+    int n = 0;
+#pragma unroll 1
+    for (int i = lane & 15; i < threads; i += 16) n += sm.before[i] <= at;
+    n = __reduce_add_sync(lane < 16 ? 0xffffu : 0xffff0000u, n) - 1;  // the last run that begins at it or before
+    cur_b = n * per;
+    int begin = sm.before[n], steps;
+    for (;;) {
+      const int2 l = cur_b < kLensCached ? sm.lens[cur_b] : load_len(p, cur_b);
+      steps = make_seq(p, l.x, l.y).steps;
+      if (at < begin + steps) break;
+      begin += steps;
+      ++cur_b;
     }
-    if (lane == 0) sm.range[warp] = x;
+    begin *= units;
+    if (pass == 0) {
+      if (ask > 0 && steps <= whole) {
+        const int in = (x - begin) % steps;
+        x += 2 * in < steps ? -in : steps - in;
+      }
+      __syncwarp();
+      const int lo = __shfl_sync(0xffffffffu, x, 0), cta_steps = __shfl_sync(0xffffffffu, x, 16) - lo;
+      if (cta_steps == 0) return;  // the whole CTA
+      // workers with steps are the first ones: their parts follow one another
+      const int each = cta_steps / H::kWarps, rem = cta_steps - each * H::kWarps;
+      x0 = x = lo + warp * each + min(warp, rem);
+      n_steps = each + (warp < rem);
+      if (n_steps == 0) x = lo;  // (asks for anything)
+      cur_b = __shfl_sync(0xffffffffu, cur_b, 0);
+      begin = __shfl_sync(0xffffffffu, begin, 0);
+      steps = __shfl_sync(0xffffffffu, steps, 0);
+      cur_rel = begin - x;
+      if (x < begin + steps * units) break;
+    } else {
+      cur_rel = begin - x;
+    }
   }
-  __syncthreads();
-  const int cta_steps = sm.range[1] - sm.range[0];
-  if (cta_steps == 0) return;  // the whole CTA
-  const Split shares(cta_steps, H::kWarps);  // (workers with steps are the first ones: their parts follow one another)
-  const int x0 = sm.range[0] + shares.begin(warp);
-  const int n_steps = sm.range[0] + shares.begin(warp + 1) - x0;
   const uint32_t worker = blockIdx.x * H::kWarps + warp;
 
   // ---- issuing: lane i knows step batch0 + i
-  int cur_b = 0, batch0 = -32;
-  int cur_rel = 0;  // first step of sequence cur_b, from the worker's first
+  int batch0 = -32;
   Step ahead{};
-  if (n_steps > 0) {
-    const Found f = find(x0);
-    cur_b = f.b;
-    cur_rel = f.begin - x0;
-  }
   auto head_of = [&](int sub) { return p.row_tiles == 1 ? sub : sub / p.row_tiles; };
   auto limit_at = [&](int len, int cnt, int n) {
     return max(len - cnt + 1 + min(token_of(p, min(n, p.rows - 1)), cnt - 1), 0);
@@ -1101,6 +1106,7 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
   if (!aligned16(workspace)) return fail(NSA_ERR_ALIGN, "workspace must be 16-byte aligned");
   if (!tickets) return fail(NSA_ERR_WORKSPACE, "tickets must not be NULL");
   p.row_tiles = s.row_tiles;
+  p.units_inv = 1.f / (float(p.c.n_kv_heads) * s.row_tiles);
   p.counts = counts;
   p.window = window < 0 ? -1 : static_cast<int>(window);
   p.sink = static_cast<int>(sink);

@@ -36,8 +36,8 @@ def _unit_at(steps, units, x):
 
 def _whole(split, steps, units):
     """Units of at most this many steps are not cut between CTAs."""
-    most = -(-len(steps) * units // split.n) * max(steps)
-    return max(steps) if most <= split.each + MERGE else 2 * MERGE
+    most = (split.each + MERGE) // max(steps)  # units of the longest kind a CTA may have
+    return max(steps) if len(steps) * units <= split.n * most else 2 * MERGE
 
 
 def _border(split, steps, units, c):
