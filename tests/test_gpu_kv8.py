@@ -527,3 +527,37 @@ def test_refusals():
         c.read(4, dtype=torch.int32)
     assert c.lens.tolist() == [0, 0]
     _clean()
+
+
+@pytest.mark.parametrize("n", [126, 127, 400])
+def test_step_equals_append_and_attend_in_every_form(n):
+    """Ragged counts, a rewind, a window, a start that is refused and one that is not; a batch beyond what the split keeps
+    at hand; repeated back to back, so that steps follow one another without a pause."""
+    hkv, group, d, t = 2, 4, 64, 3
+    for b in (4, 700):
+        k, v = _tokens(b, hkv, n + 4 * t, d, BF16, 40)
+        one, two = (pkg.Kv8Cache(b, hkv, n + 4 * t, head_dim=d, dtype=BF16, device=DEV) for _ in range(2))
+        lens = [(n - 7 * i) % n + 1 for i in range(b)]
+        for c in (one, two):
+            _fill(c, k, v, lens)
+        counts = torch.tensor([i % (t + 1) for i in range(b)], device=DEV)
+        starts = torch.tensor(lens, device=DEV)
+        starts[0] = -3  # refused: this sequence stays as it is
+        starts[1] = lens[1] // 64 * 64
+        q = _queries(b, hkv * group, t, d, BF16, 41)
+        nk, nv = k[:, :, n:n + t], v[:, :, n:n + t]
+        pairs = []
+        for i in range(4):
+            kw = dict(counts=counts, starts=starts if i % 2 == 0 else None)
+            mask = dict(window=50, sink=2) if i > 1 else {}
+            o = one.decode_step(q, nk, nv, **kw, **mask)
+            two.append(nk, nv, **kw)
+            pairs.append((o, two.attend(q, counts=counts, **mask), one.lens.clone(), two.lens.clone()))
+        for o, p, a, c in pairs:
+            assert torch.equal(o, p) and torch.equal(a, c)
+        assert pkg.device_error(torch.device(DEV)) == 1
+        assert one.lens[0] == lens[0] + 0 and one.lens.tolist()[1:3] == two.lens.tolist()[1:3]
+        for x in ("k_ring", "v_ring", "scales", "_ring_floor"):
+            assert torch.equal(getattr(one, x), getattr(two, x)), x
+        assert torch.equal(one.k_codes.view(torch.uint8), two.k_codes.view(torch.uint8))
+        assert not one._append_tickets.any() and not two._append_tickets.any()
