@@ -10,10 +10,14 @@
 // into [1, 2): exact for fp16 and for bf16 but for elements 2^-14 below the
 // row's largest, which keep an absolute error of 2^-25 of it.
 //
-// Bound by HBM for up to about 32 query rows a KV head: 8 rows take 16 FLOP a
-// byte.  tcgen05 would want the codes as fp16 in shared memory first and tiles
-// of 64 or 128 rows; here the conversion happens in registers on the way from
-// ldmatrix to the mma.
+// Bound by HBM for up to 8 query rows a KV head, which take 16 FLOP a byte (4 x
+// 163,840 tokens, 64 / 8 heads of 128: 214 us, 0.96 of the measured copy rate); by
+// the instructions around the products for more (32 rows: 0.31).  tcgen05 would
+// want the codes as fp16 in shared memory first and tiles of 64 or 128 rows; here
+// the conversion happens in registers on the way from ldmatrix to the mma.
+// Short calls are bound by the way from the lengths to the first load (3 us from
+// the launch to the page number, 2 more to its keys) and by one step's
+// latency (2.6 us); B = 1, L = 512 takes 10 us.
 //
 // Work is split evenly over independent workers (warps) by steps: a step is a
 // block of 64 tokens, or 32 tokens of a sequence's incomplete block in the

@@ -7,7 +7,8 @@
 // throughout, so the codes are reproducible to the bit.  Bound by HBM: 2 bytes
 // in and 1 byte out per element.  One CTA holds a whole block of K and of V in
 // registers (8 K + 8 V elements a thread and row), so the tokens are read once
-// for both the maximum and the codes.
+// for both the maximum and the codes.  16 prompts of 8000 tokens, 8 heads of 128,
+// bf16: 127 us, 0.95 of the measured copy rate.
 #include <cstdlib>
 
 #include "kv8.cuh"
@@ -269,7 +270,10 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
 
 // The same for fewer new tokens than a block has, a smaller CTA a unit: most
 // units only store a row or a few, so what counts is how many CTAs are resident
-// at once; K and V of a block that is completed take turns in the registers.
+// at once; K and V of a block that is completed take turns in the registers (40
+// of them: 6 CTAs an SM).  One token of 256 x 8 units: 6.2 us, 7.3 with the
+// kernel above; 256 units that all complete a block: 2 us more than there (with
+// 128 threads 5.7 us and 4 more, with 64 and the block read twice 12 and 30).
 constexpr int kFewThreads = 256;
 template <int kD, bool kBf16, bool kInt8>
 __global__ void __launch_bounds__(kFewThreads) kv8_append_few_kernel(const AppendParams p) {
@@ -371,7 +375,9 @@ __device__ __forceinline__ void store16(void* out, int64_t at, const float (&x)[
 
 // One CTA a tile of kReadRows positions of a unit; a thread takes 16 elements of a
 // row of K and of V.  Bound by HBM (1 byte in, 2 out an element): all of a
-// thread's loads are issued before its stores.
+// thread's loads are issued before its stores.  8 x 16,000 tokens, 8 heads of 128
+// to bf16: 146 us, 0.83 of the measured copy rate (128 rows a CTA: 150; stores
+// that bypass the L2: the same).
 constexpr int kReadRows = 64;
 template <int kD, bool kBf16, bool kInt8, int kOut>
 __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const ReadParams p) {
