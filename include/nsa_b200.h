@@ -345,7 +345,8 @@ int64_t nsa_kv8_ticket_count(void);
 int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_kv8_rows* o, int64_t n_heads,
                    int64_t n_tokens, const int64_t* counts, int64_t window, int64_t sink, float sm_scale,
                    void* workspace, size_t workspace_bytes, int32_t* tickets, nsa_stream_t stream);
-/* nsa_kv8_append of the n_tokens, then nsa_kv8_attend of their queries. */
+/* nsa_kv8_append of the n_tokens, then nsa_kv8_attend of their queries;
+ * nothing is written when an argument of either is refused. */
 int nsa_kv8_decode_step(const nsa_kv8_cache* cache, const nsa_kv8_rows* new_k, const nsa_kv8_rows* new_v,
                         const nsa_kv8_rows* q, const nsa_kv8_rows* o, int64_t n_heads, int64_t n_tokens,
                         const int64_t* starts, const int64_t* counts, int64_t window, int64_t sink, float sm_scale,

@@ -220,7 +220,8 @@ __device__ __forceinline__ void to_half(uint32_t w, uint32_t& lo, uint32_t& hi) 
 }
 
 __device__ __forceinline__ void lds8(uint32_t addr, uint32_t& lo, uint32_t& hi) {
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo), "=r"(hi) : "r"(addr));
+  // (memory: it may read what plain stores have written)
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo), "=r"(hi) : "r"(addr) : "memory");
 }
 // A pair of fp16 numbers of 8 significant bits as bf16 (exact).  volatile, so
 // that the conversions of all query fragments stay on the ring's path instead
@@ -1085,10 +1086,21 @@ size_t nsa_kv8_workspace_bytes(const nsa_kv8_cache* cache, int64_t n_heads, int6
   return kv8::plan(cache, n_heads / cache->n_kv_heads * n_tokens).bytes;
 }
 
-int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_kv8_rows* o, int64_t n_heads,
-                   int64_t n_tokens, const int64_t* counts, int64_t window, int64_t sink, float sm_scale,
-                   void* workspace, size_t workspace_bytes, int32_t* tickets, nsa_stream_t stream) {
-  clear_error();
+}  // extern "C"
+
+namespace {
+
+// The append that comes with an attention in a decode step.
+struct Append {
+  const nsa_kv8_rows *new_k, *new_v;
+  const int64_t* starts;
+};
+
+// Checks an attention's arguments, then runs the append (if any; nothing is
+// written when an argument of either is refused) and launches the attention.
+int attend(const nsa_kv8_cache* cache, const Append* add, const nsa_kv8_rows* q, const nsa_kv8_rows* o, int64_t n_heads,
+           int64_t n_tokens, const int64_t* counts, int64_t window, int64_t sink, float sm_scale, void* workspace,
+           size_t workspace_bytes, int32_t* tickets, nsa_stream_t stream) {
   kv8::AttendParams p{};
   int rc = kv8::check_cache(cache, p.c);
   if (rc) return rc;
@@ -1135,6 +1147,7 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
                               CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
   }
+  if (add && (rc = nsa_kv8_append(cache, add->new_k, add->new_v, n_tokens, add->starts, counts, stream))) return rc;
   const bool bf16 = cache->dtype == 2, int8 = cache->codes == NSA_KV8_INT8;
   if (d == 128)
     return bf16 ? (int8 ? kv8::launch_rows<128, true, true>(s, maps, p, stream)
@@ -1147,14 +1160,26 @@ int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_
                       : kv8::launch_rows<64, false, false>(s, maps, p, stream));
 }
 
+}  // namespace
+
+extern "C" {
+
+int nsa_kv8_attend(const nsa_kv8_cache* cache, const nsa_kv8_rows* q, const nsa_kv8_rows* o, int64_t n_heads,
+                   int64_t n_tokens, const int64_t* counts, int64_t window, int64_t sink, float sm_scale,
+                   void* workspace, size_t workspace_bytes, int32_t* tickets, nsa_stream_t stream) {
+  clear_error();
+  return attend(cache, nullptr, q, o, n_heads, n_tokens, counts, window, sink, sm_scale, workspace, workspace_bytes,
+                tickets, stream);
+}
+
 int nsa_kv8_decode_step(const nsa_kv8_cache* cache, const nsa_kv8_rows* new_k, const nsa_kv8_rows* new_v,
                         const nsa_kv8_rows* q, const nsa_kv8_rows* o, int64_t n_heads, int64_t n_tokens,
                         const int64_t* starts, const int64_t* counts, int64_t window, int64_t sink, float sm_scale,
                         void* workspace, size_t workspace_bytes, int32_t* tickets, nsa_stream_t stream) {
-  const int rc = nsa_kv8_append(cache, new_k, new_v, n_tokens, starts, counts, stream);
-  if (rc) return rc;
-  return nsa_kv8_attend(cache, q, o, n_heads, n_tokens, counts, window, sink, sm_scale, workspace, workspace_bytes,
-                        tickets, stream);
+  clear_error();
+  const Append add{new_k, new_v, starts};
+  return attend(cache, &add, q, o, n_heads, n_tokens, counts, window, sink, sm_scale, workspace, workspace_bytes,
+                tickets, stream);
 }
 
 }  // extern "C"

@@ -525,7 +525,11 @@ def test_refusals():
         c.decode_step(q, new[:, :, None].expand(2, 2, 3, 128), new)
     with pytest.raises(TypeError):
         c.read(4, dtype=torch.int32)
-    assert c.lens.tolist() == [0, 0]
+    with pytest.raises(ValueError, match="finite"):
+        c.decode_step(q, new, new, sm_scale=float("inf"))  # and nothing is appended
+    with pytest.raises(ValueError, match="aligned"):
+        c.decode_step(q, new, torch.zeros(2 * 2 * 128 + 1, dtype=F16, device=DEV)[1:].view(2, 2, 128))
+    assert c.lens.tolist() == [0, 0] and not c.k_ring.any()
     _clean()
 
 

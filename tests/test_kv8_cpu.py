@@ -115,5 +115,9 @@ def test_arguments_are_checked():
     assert attend(window=1 << 40) == 1 and attend(scale=float("inf")) == 1 and attend(scale=float("nan")) == 1
     assert attend(ws=None) == 4 and attend(n=16) == 4 and attend(tickets=None) == 4 and attend(ws=4100) == 2
     assert attend(desc=_desc(batch=0), q=None) == 0
+    def step(k=r, v=r, scale=0.1, ws=4096):
+        return lib.nsa_kv8_decode_step(d, k, v, r, r, 4, 1, None, None, -1, 4, scale, ws, 1 << 30, 4096, None)
+
+    assert step(scale=float("nan")) == 1 and step(ws=None) == 4
     assert lib.nsa_kv8_ticket_count() > 0 and lib.nsa_kv8_workspace_bytes(d, 4, 1) > 0
     assert lib.nsa_kv8_workspace_bytes(d, 4, 65) == 0
