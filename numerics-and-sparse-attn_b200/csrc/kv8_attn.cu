@@ -29,7 +29,6 @@
 // (sequence, KV head, row tile).  Units cut between workers are merged by the
 // CTA at its end, and those cut between CTAs by the last of them to finish.
 #include <cstddef>
-#include <cstdlib>
 
 #include "kv8.cuh"
 
@@ -141,7 +140,7 @@ struct Part {
 // One CTA per SM.  12 warps of 168 registers where the accumulators leave room
 // (up to 8 query rows of 128 dimensions, 16 of 64), else 8 of 255.  Spilled
 // registers are dear here: with this much shared memory they miss the L1.
-template <int kD, int kNT, bool kSplit>
+template <int kD, int kNT>
 struct Shape {
   static constexpr int kWarps = kNT * kD <= 128 ? 12 : 8;
   static constexpr int kThreads = kWarps * 32;
@@ -150,9 +149,9 @@ struct Shape {
   static constexpr int kTok = 32;  // tokens of a round of scores, softmax and sums
 };
 
-template <int kD, int kNT, bool kSplit>
+template <int kD, int kNT>
 struct Smem {
-  using H = Shape<kD, kNT, kSplit>;
+  using H = Shape<kD, kNT>;
   uint8_t stage[H::kWarps][2 * Geo<kD>::kHalf];  // K, V; 1024-aligned: TMA destinations
   uint8_t q[H::kWarps][H::kRows][H::kQStride];
   Part part[H::kWarps][2];
@@ -311,7 +310,7 @@ __device__ __forceinline__ void merge_row(int n, int row, int lane, Ptr ptr, flo
 }
 
 template <int kD, int kNT, bool kBf16, bool kInt8>
-__global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
+__global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
     kv8_attend_kernel(const __grid_constant__ CUtensorMap tm_kc, const __grid_constant__ CUtensorMap tm_vc,
                       const __grid_constant__ CUtensorMap tm_kr, const __grid_constant__ CUtensorMap tm_vr,
                       const AttendParams p) {
@@ -320,8 +319,8 @@ __global__ void __launch_bounds__(Shape<kD, kNT, !kBf16>::kThreads, 1)
   // the output to fp16 makes, and far below bf16's.  With fp16 outputs P is
   // the sum of two fp16 numbers (2^-23).
   constexpr bool kSplitP = !kBf16;
-  using H = Shape<kD, kNT, kSplitP>;
-  using S = Smem<kD, kNT, kSplitP>;
+  using H = Shape<kD, kNT>;
+  using S = Smem<kD, kNT>;
   constexpr int kRows = H::kRows;
   constexpr int kChunks = kD / 16;              // 16-wide steps of the head dimension
   constexpr int kTC = H::kTok / 16;             // 16-token parts of a round
@@ -1023,7 +1022,7 @@ Plan plan(const nsa_kv8_cache* c, int64_t rows) {
   Plan s;
   s.nt = rows <= 8 ? 1 : 2;
   const int tile = 8 * s.nt;
-  const int workers = s.nt * c->head_dim <= 128 ? Shape<128, 1, true>::kWarps : Shape<128, 2, true>::kWarps;
+  const int workers = s.nt * c->head_dim <= 128 ? Shape<128, 1>::kWarps : Shape<128, 2>::kWarps;
   s.row_tiles = static_cast<int>((rows + tile - 1) / tile);
   const int64_t most = c->batch * c->n_kv_heads * s.row_tiles * (c->max_blocks + 2);  // steps
   s.n_ctas = static_cast<int>(most < max_ctas() ? most : max_ctas());
@@ -1033,8 +1032,8 @@ Plan plan(const nsa_kv8_cache* c, int64_t rows) {
 
 template <int kD, int kNT, bool kBf16, bool kInt8>
 int launch_attend(const Plan& plan, const CUtensorMap (&maps)[4], const AttendParams& p, cudaStream_t stream) {
-  using S = Smem<kD, kNT, !kBf16>;
-  using H = Shape<kD, kNT, !kBf16>;
+  using S = Smem<kD, kNT>;
+  using H = Shape<kD, kNT>;
   static_assert(offsetof(S, stage) == 0 && Geo<kD>::kHalf % 1024 == 0, "TMA destinations");
   static_assert(offsetof(S, q) % 16 == 0, "vector reads");
   static_assert(sizeof(S) <= 227 * 1024, "shared memory of an SM");

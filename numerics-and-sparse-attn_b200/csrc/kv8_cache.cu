@@ -9,7 +9,6 @@
 // registers (8 K + 8 V elements a thread and row), so the tokens are read once
 // for both the maximum and the codes.  16 prompts of 8000 tokens, 8 heads of 128,
 // bf16: 127 us, 0.95 of the measured copy rate.
-#include <cstdlib>
 
 #include "kv8.cuh"
 
@@ -149,7 +148,11 @@ __device__ __forceinline__ Span take_span(const AppendParams& p, int b, int aske
   const bool ok = s >= 0 && s <= len && len <= cap && n >= 0 && n <= p.n_tokens && s + n <= cap &&
                   (s % kBlock == 0 || s >= floor);
   if (!ok) set_error(p.err, NSA_ERR_INVALID);
-  if (atomicAdd(c.tickets + b, 1) == askers - 1) {
+  // The ticket's step is made from `ok` (the same for all of a sequence's askers):
+  // it cannot be taken before what this thread needs of lens and floor is there.
+  // (A fence in its place costs 0.8 us a call, 13 us in a prompt of 8000 tokens.)
+  const int step = ok ? 1 : 2;
+  if (atomicAdd(c.tickets + b, step) == (askers - 1) * step) {
     c.tickets[b] = 0;
     if (ok) {
       const int64_t first = s / kBlock * kBlock, last = (s + n) / kBlock * kBlock;
@@ -462,7 +465,9 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
                          0, stream, p);
   }
   const int more = (p.n_tokens + kBlock - 1) / kBlock;  // blocks besides a unit's first
-  const dim3 grid(static_cast<unsigned>(units), 1 + static_cast<unsigned>(more < 65534 ? more : 65534));
+  int most = (1 << 30) / p.c.n_kv_heads - 2;  // twice a sequence's CTAs is an int
+  most = most < 65534 ? most : 65534;
+  const dim3 grid(static_cast<unsigned>(units), 1 + static_cast<unsigned>(more < most ? more : most));
   return launch_kernel(kv8_append_kernel<kD, kBf16, kInt8>, grid, dim3(kThreads), 0, stream, p);
 }
 template <int kD, bool kBf16, bool kInt8>

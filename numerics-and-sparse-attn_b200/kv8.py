@@ -49,8 +49,16 @@ def _graph_rows(device):
             _graph[device.index] = [torch.zeros((_GRAPH_ROWS, n), dtype=torch.int32, device=device), 0]
 
 
+def _capturing(index):
+    """Whether the device's current stream is being captured."""
+    if torch._C._cuda_getDevice() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def _scratch(device, nbytes, stream):
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing(device.index):
         with _scratch_lock:
             slot = _graph[device.index]
             row = slot[1]
@@ -140,6 +148,7 @@ class Kv8Cache:
         _req(device.type == "cuda", "Kv8Cache lives on a CUDA device (no CPU fallback)")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
+        _req(not _capturing(device.index), "a Kv8Cache cannot be made while a graph is captured", RuntimeError)
         self.batch, self.n_kv_heads, self.head_dim, self.dtype, self.codes = batch, n_kv_heads, head_dim, dtype, codes
         self.max_blocks = (max_len + BLOCK - 1) // BLOCK
         self.n_pages = max(1, batch * self.max_blocks) if n_pages is None else int(n_pages)
@@ -242,6 +251,7 @@ class Kv8Cache:
     def truncate(self, lens):
         """Set the lengths to ``lens`` (int64 [B]), taking tokens back as
         ``append``'s ``starts`` does (0 empties a sequence)."""
+        _req(lens is not None, "lens must be a tensor")
         self._call(self._lib.nsa_kv8_append, None, None, 0, self._words("lens", lens), None)
 
     # ---------------------------------------------------------------- reading

@@ -383,6 +383,19 @@ def test_bf16_range(factor):
     _clean()
 
 
+@pytest.mark.parametrize("scale", [-0.1, 0.0, 3.0])
+def test_scales_of_any_sign(scale):
+    b, hkv, group, d = 2, 2, 4, 128
+    lens = [200, 67]
+    k, v = _tokens(b, hkv, 200, d, F16, 71)
+    cache = pkg.Kv8Cache(b, hkv, 200, device=DEV)
+    _fill(cache, k, v, lens)
+    q = _queries(b, hkv * group, 2, d, F16, 72)
+    scale = torch.tensor(scale, dtype=torch.float32).item()
+    _check_attend(cache, cache.attend(q, sm_scale=scale), q, k, v, lens, scale=scale)
+    _clean()
+
+
 def test_zero_blocks_and_zero_queries():
     k = torch.zeros(2, 1, 130, 64, dtype=F16, device=DEV)
     v = k.clone()
@@ -525,6 +538,8 @@ def test_refusals():
         c.decode_step(q, new[:, :, None].expand(2, 2, 3, 128), new)
     with pytest.raises(TypeError):
         c.read(4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="lens"):
+        c.truncate(None)
     with pytest.raises(ValueError, match="finite"):
         c.decode_step(q, new, new, sm_scale=float("inf"))  # and nothing is appended
     with pytest.raises(ValueError, match="aligned"):
