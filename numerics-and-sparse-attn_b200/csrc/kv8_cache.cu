@@ -361,30 +361,28 @@ __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
 
 // kOut: 0 float32, 1 float16, 2 bfloat16
 template <int kOut>
-__device__ __forceinline__ void store16(void* out, int64_t at, const float (&x)[16]) {
+__device__ __forceinline__ void store8(void* out, int64_t at, const float (&x)[8]) {
   if constexpr (kOut == 0) {
     float4* o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    o[0] = make_float4(x[0], x[1], x[2], x[3]);
+    o[1] = make_float4(x[4], x[5], x[6], x[7]);
   } else {
-    uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at);
     using E = Elem<kOut == 2>;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      o[i] = make_uint4(E::pack(x[8 * i], x[8 * i + 1]), E::pack(x[8 * i + 2], x[8 * i + 3]),
-                        E::pack(x[8 * i + 4], x[8 * i + 5]), E::pack(x[8 * i + 6], x[8 * i + 7]));
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) =
+        make_uint4(E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(x[4], x[5]), E::pack(x[6], x[7]));
   }
 }
 
-// One CTA a tile of kReadRows positions of a unit; a thread takes 16 elements of a
-// row of K and of V.  Bound by HBM (1 byte in, 2 out an element): all of a
-// thread's loads are issued before its stores.  8 x 16,000 tokens, 8 heads of 128
-// to bf16: 146 us, 0.83 of the measured copy rate (128 rows a CTA: 150; stores
-// that bypass the L2: the same).
+// One CTA a tile of kReadRows positions of a unit; a thread takes 8 elements of a
+// row of K and of V, so that a warp's 16-byte stores fill whole sectors.  Bound
+// by HBM (1 byte in, 2 out an element): all of a thread's loads are issued before
+// its stores.  8 x 16,000 tokens, 8 heads of 128 to bf16: 123 us, 0.99 of the
+// measured copy rate (16 elements a thread, each store half a sector a lane: 146;
+// CTAs that take tiles in turn and look the next one's pages up ahead: 166).
 constexpr int kReadRows = 64;
 template <int kD, bool kBf16, bool kInt8, int kOut>
 __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const ReadParams p) {
-  constexpr int kVecs = kD / 16, kRowsPass = kThreads / kVecs, kN = kReadRows / kRowsPass;
+  constexpr int kVecs = kD / 8, kRowsPass = kThreads / kVecs, kN = kReadRows / kRowsPass;
   grid_launch_dependents();
   grid_dependency_wait();
   const Cache& c = p.c;
@@ -398,13 +396,13 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const ReadParams p) 
   }
   const int64_t start = p.starts ? p.starts[b] : 0;
   const int64_t full = len / kBlock * kBlock;  // positions below are codes
-  const int col = (threadIdx.x % kVecs) * 16, row0 = threadIdx.x / kVecs;
-  uint4 kc[kN], vc[kN];
+  const int col = (threadIdx.x % kVecs) * 8, row0 = threadIdx.x / kVecs;
+  uint2 kc[kN], vc[kN];
   float2 sc[kN];
 #pragma unroll
   for (int j = 0; j < kN; ++j) {
     const int64_t r = tile * kReadRows + row0 + j * kRowsPass, pos = start + r;
-    kc[j] = vc[j] = make_uint4(0, 0, 0, 0);
+    kc[j] = vc[j] = make_uint2(0, 0);
     sc[j] = make_float2(0.f, 0.f);
     if (r < p.n_tokens && pos >= 0 && pos < full) {
       const int page = __ldg(c.page_table + int64_t(b) * c.max_blocks + pos / kBlock);
@@ -413,8 +411,8 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const ReadParams p) 
         sc[j] = make_float2(NAN, NAN);
       } else {
         const int64_t rec = int64_t(page) * c.n_kv_heads + h, at = (rec * kBlock + pos % kBlock) * kD + col;
-        kc[j] = __ldg(reinterpret_cast<const uint4*>(c.k_codes + at));
-        vc[j] = __ldg(reinterpret_cast<const uint4*>(c.v_codes + at));
+        kc[j] = __ldg(reinterpret_cast<const uint2*>(c.k_codes + at));
+        vc[j] = __ldg(reinterpret_cast<const uint2*>(c.v_codes + at));
         sc[j] = __ldg(c.scales + rec);
       }
     }
@@ -426,33 +424,29 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(const ReadParams p) 
     const int64_t at = (unit * p.n_tokens + r) * kD + col;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      float x[16];
+      float x[8];
       if (pos >= full && pos < len) {
-        const uint4* src = reinterpret_cast<const uint4*>((t ? c.v_ring : c.k_ring) +
-                                                          (unit * kRing + pos % kRing) * kD + col);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 w = __ldg(src + i);
-          const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = Elem<kBf16>::unpack(ws[e]);
-            x[8 * i + 2 * e] = f.x, x[8 * i + 2 * e + 1] = f.y;
-          }
-        }
-      } else {
-        const uint4 w = t ? vc[j] : kc[j];
-        const float s = t ? sc[j].y : sc[j].x;
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>((t ? c.v_ring : c.k_ring) +
+                                                             (unit * kRing + pos % kRing) * kD + col));
         const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int e = 0; e < 4; ++e) {
+          const float2 f = Elem<kBf16>::unpack(ws[e]);
+          x[2 * e] = f.x, x[2 * e + 1] = f.y;
+        }
+      } else {
+        const uint2 w = t ? vc[j] : kc[j];
+        const float s = t ? sc[j].y : sc[j].x;
+        const uint32_t ws[2] = {w.x, w.y};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
           float y[4];
           decode4<kInt8>(ws[i], y);
 #pragma unroll
           for (int e = 0; e < 4; ++e) x[4 * i + e] = y[e] * s;
         }
       }
-      store16<kOut>(t ? p.v_out : p.k_out, at, x);
+      store8<kOut>(t ? p.v_out : p.k_out, at, x);
     }
   }
 }
