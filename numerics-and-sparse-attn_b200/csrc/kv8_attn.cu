@@ -315,10 +315,6 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
                       const __grid_constant__ CUtensorMap tm_kr, const __grid_constant__ CUtensorMap tm_vr,
                       const AttendParams p) {
   using G = Geo<kD>;
-  // P as one fp16 number has a relative error of 2^-12, the same as rounding
-  // the output to fp16 makes, and far below bf16's.  With fp16 outputs P is
-  // the sum of two fp16 numbers (2^-23).
-  constexpr bool kSplitP = !kBf16;
   using H = Shape<kD, kNT>;
   using S = Smem<kD, kNT>;
   constexpr int kRows = H::kRows;
@@ -750,23 +746,20 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
             const float p2 = fast_exp2(sc[i][nt][2] - ref[0]), p3 = fast_exp2(sc[i][nt][3] - ref[1]);
             l[nt][0] += p0 + p2;
             l[nt][1] += p1 + p3;
-            uint32_t hi0, hi1, lo0 = 0, lo1 = 0;
+            uint32_t hi0, hi1, lo0, lo1;
+            // P in two parts: as one fp16 number it would add 2^-11 to an output's rounding, which is 2^-11
+            // itself in fp16 and 2^-8 in bf16 (and changes a bf16 output's last place in 1 of 40).
             if (kBf16 && ring) {
               split_pair<true>(p0, p1, hi0, lo0);
               split_pair<true>(p2, p3, hi1, lo1);
-            } else if (kSplitP) {
+            } else {
               split_pair<false>(p0, p1, hi0, lo0);
               split_pair<false>(p2, p3, hi1, lo1);
-            } else {
-              hi0 = pack_half2(p0, p1);
-              hi1 = pack_half2(p2, p3);
             }
             pb[i][nt][0] = movmatrix_trans(hi0);  // rows 2t, 2t + 1 of the tokens, query row g
             pb[i][nt][1] = movmatrix_trans(hi1);  // and 2t + 8, 2t + 9
-            if (kSplitP || (ring && i < kRC)) {
-              pl[i][nt][0] = movmatrix_trans(lo0);
-              pl[i][nt][1] = movmatrix_trans(lo1);
-            }
+            pl[i][nt][0] = movmatrix_trans(lo0);
+            pl[i][nt][1] = movmatrix_trans(lo1);
           }
         }
         if (__any_sync(0xffffffffu, moved)) {
@@ -800,7 +793,7 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
                     mma_first(blk[j][nt], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
                   else
                     mma_16816(blk[j][nt], a0, a1, a2, a3, pb[i][nt][0], pb[i][nt][1]);
-                  if constexpr (kSplitP) mma_16816(blk[j][nt], a0, a1, a2, a3, pl[i][nt][0], pl[i][nt][1]);
+                  mma_16816(blk[j][nt], a0, a1, a2, a3, pl[i][nt][0], pl[i][nt][1]);
                 }
               }
             }

@@ -76,9 +76,9 @@ def bound(o, spread, reach, dtype, d):
     * a score is a sum of d products with float32 rounding (2^-24 each, some more for its scaling and exponential
       argument): d + 16 roundings of at most `reach`; softmax weights then move by at most twice that, relatively;
     * the exponential itself and the sums: 2^-20;
-    * P rounded to fp16 (eps / 2 = 2^-11) where the output is bfloat16; in two parts (2^-22) where it is float16;
+    * P in two fp16 parts (2^-22), in two bfloat16 ones (2^-18) beside 16-bit tokens of bfloat16;
     * an element below the type's smallest normal number: its absolute step."""
     fi = torch.finfo(dtype)
-    p_err = 2.0 ** -11 if dtype == torch.bfloat16 else 2.0 ** -22
+    p_err = 2.0 ** -18 if dtype == torch.bfloat16 else 2.0 ** -22
     rel = 2 * (d + 16) * 2.0 ** -24 * reach + 2.0 ** -20 + p_err
     return fi.eps / 2 * o.abs() * (1 + 1e-3) + rel * spread * (1 + fi.eps) + fi.smallest_normal * fi.eps

@@ -1,0 +1,53 @@
+"""Softmax weights of the 8-bit cache's attention (Kv8Cache.attend) where the
+precision that they are held in shows: each weight's own output element, within
+half a step of the output's type.
+
+Queries have one element other than 0, so that a score is one product and has
+no rounding of a sum of D of them.  Its roundings in float32, each at most
+2^-24 of it: of scale * log2(e) (two), of the block's and the query's scale
+(two), of the product, of the distance to the maximum; a weight moves by twice
+6 * 2^-24 * |score| (numerator and denominator) at most."""
+import importlib
+
+import pytest
+import torch
+
+from oracle import kv8 as ok
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+pkg = importlib.import_module("numerics-and-sparse-attn_b200")
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _half_step(x, dtype):
+    """Half the distance of the type's numbers around x, element by element."""
+    fi = torch.finfo(dtype)
+    _, e = torch.frexp(x.abs().clamp_min(fi.smallest_normal))
+    return torch.ldexp(torch.full_like(x, fi.eps / 4), e)  # x = f 2^e, 0.5 <= f < 1
+
+
+@pytest.mark.parametrize("n", [64, 63])  # a block of codes; the 16-bit tokens
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("codes", ["e4m3", "int8"])
+def test_every_weight_is_right_to_half_a_step_of_the_output(dtype, codes, n):
+    """V is the unit matrix: output element j is token j's weight.  A weight held in as many bits as the output adds
+    errors of its own and misses the nearest number at every tenth element or so."""
+    b, hkv, group, d = 24, 2, 4, 64
+    g = torch.Generator(device=DEV).manual_seed(50)
+    k, v = torch.zeros(2, b, hkv, n, d, dtype=dtype, device=DEV)
+    k[..., 0] = (2 * torch.rand(b, hkv, n, device=DEV, generator=g) - 1).to(dtype)  # scores within 4 of one another
+    v[...] = torch.eye(d, device=DEV)[:n].to(dtype)
+    q = torch.zeros(b, hkv * group, d, dtype=dtype, device=DEV)
+    q[..., 0] = (0.5 + 1.5 * torch.rand(b, hkv * group, device=DEV, generator=g)).to(dtype)
+    cache = pkg.Kv8Cache(b, hkv, 64, head_dim=d, dtype=dtype, codes=codes, device=DEV)
+    cache.append(k, v)
+    o = cache.attend(q, sm_scale=1.0)
+    for i in range(b):
+        kk, vv = ok.held(k[i], n, codes), ok.held(v[i], n, codes)
+        ref, spread, reach = ok.attend(q[i][:, None], kk, vv, 1, 1.0)
+        # weights in two parts (2^-18 where they are bfloat16), the exponentials and sums 2^-20 each
+        rel = 2 * 6 * 2.0 ** -24 * reach + 2.0 ** -18 + 2 * 2.0 ** -20
+        far = (o[i].double() - ref[:, 0]).abs() - _half_step(ref, dtype)[:, 0] - (rel * spread)[:, 0]
+        assert far.max().item() <= 0, (i, far.max().item(), (far > 0).double().mean().item())
+    assert pkg.device_error(torch.device(DEV)) == 0
