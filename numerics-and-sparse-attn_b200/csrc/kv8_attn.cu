@@ -717,8 +717,18 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
                 if ((ring && i >= kRC) || !sees(p, pos0 + 16 * i + (e < 2 ? g : hi), limit)) sc[i][nt][e] = -INFINITY;
             }
         }
-        // ---- online softmax, and P as B fragments
-        float alpha[kNT][2], row_vs[kNT][2];
+        // ---- online softmax, and P as B fragments.  A round's weights are taken
+        // relative to its own maximum x and times 2^15, P = 2^(s - x + 15), which
+        // uses fp16 from its top on: with the low part, a weight has an error of
+        // 2^-22, or of 2^-40 of the round's largest if that is more.  (Relative to
+        // the maximum m so far, a long tail of weights below 2^-25 of one large
+        // weight would vanish from the sums, but not from l.)  share = 2^(x - 15 - m)
+        // brings the round's sums to m.  The bf16 parts beside bf16 tokens have the
+        // range, and those tokens' sums no room for 2^15.
+        const float raise = kBf16 && ring ? 0.f : 15.f;
+        float alpha[kNT][2], share[kNT][2], row_vs[kNT][2];
+        // vs * share of a bf16 block with tiny values would be subnormal: they are multiplied in turn
+        const bool tiny = kBf16 && s.vs < 0x1p-60f;
         uint32_t pb[kTC][kNT][2], pl[kTC][kNT][2];
         bool moved = false;
 #pragma unroll
@@ -731,21 +741,24 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
             for (int i = 0; i < kTC; ++i) x = fmaxf(x, fmaxf(sc[i][nt][e], sc[i][nt][2 + e]));
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
+            const bool none = x == -INFINITY;
+            const float mn = fmaxf(m[nt][e], x), to = mn == -INFINITY ? 0.f : mn;
+            // (from 2^20 on x - 15 would be rounded: P as it is; a maximum of 2^15.1 at most is left below 65504)
+            ref[e] = none ? 0.f : fabsf(x) < 0x1p20f ? x - raise : x;
+            share[nt][e] = none ? 0.f : fast_exp2(ref[e] - to);
             // a row that sees nothing of this block takes nothing of it, not even a scale that is NaN
-            row_vs[nt][e] = x == -INFINITY ? 0.f : s.vs;
-            const float mn = fmaxf(m[nt][e], x);
-            ref[e] = mn == -INFINITY ? 0.f : mn;
-            alpha[nt][e] = fast_exp2(m[nt][e] - ref[e]);
+            row_vs[nt][e] = none ? 0.f : tiny ? s.vs : s.vs * share[nt][e];
+            alpha[nt][e] = fast_exp2(m[nt][e] - to);
             moved |= alpha[nt][e] != 1.f;
             m[nt][e] = mn;
-            l[nt][e] *= alpha[nt][e];
           }
+          float sum[2] = {0.f, 0.f};
 #pragma unroll
           for (int i = 0; i < kTC; ++i) {
             const float p0 = fast_exp2(sc[i][nt][0] - ref[0]), p1 = fast_exp2(sc[i][nt][1] - ref[1]);
             const float p2 = fast_exp2(sc[i][nt][2] - ref[0]), p3 = fast_exp2(sc[i][nt][3] - ref[1]);
-            l[nt][0] += p0 + p2;
-            l[nt][1] += p1 + p3;
+            sum[0] += p0 + p2;
+            sum[1] += p1 + p3;
             uint32_t hi0, hi1, lo0, lo1;
             // P in two parts: as one fp16 number it would add 2^-11 to an output's rounding, which is 2^-11
             // itself in fp16 and 2^-8 in bf16 (and changes a bf16 output's last place in 1 of 40).
@@ -761,6 +774,8 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
             pl[i][nt][0] = movmatrix_trans(lo0);
             pl[i][nt][1] = movmatrix_trans(lo1);
           }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) l[nt][e] = l[nt][e] * alpha[nt][e] + sum[e] * share[nt][e];
         }
         if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
@@ -770,7 +785,7 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[nt][c][e] *= alpha[nt][e & 1];
         }
-        // ---- O^T += vs V^T P^T
+        // ---- O^T += share vs V^T P^T
         if (round == 0 && !aborted && !mbar_wait(smem_u32(&sm.v_full[warp]), k & 1, p.err)) aborted = true;
         if (!ring) {
           const uint32_t va = vb + v_off + round * H::kTok * kD;
@@ -797,6 +812,17 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
                 }
               }
             }
+            if (tiny) {
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    blk[j][nt][e] *= share[nt][e & 1];
+                    asm volatile("" : "+f"(blk[j][nt][e]));  // (a branch: predicated, all rounds would issue these)
+                  }
+            }
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -805,6 +831,7 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
                 for (int e = 0; e < 4; ++e) acc[nt][c + j][e] += row_vs[nt][e & 1] * blk[j][nt][e];
           }
         } else {
+          // (a sum of its own for each 16 tokens: it has to be weighted, and one for both would take more registers)
 #pragma unroll
           for (int i = 0; i < kRC; ++i) {
             const int tok0 = round * H::kTok + 16 * i;
@@ -852,8 +879,11 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
               }
 #pragma unroll
               for (int nt = 0; nt < kNT; ++nt) {
-                mma_elem<kBf16>(acc[nt][c], a[0], a[1], a[2], a[3], pb[i][nt][0], pb[i][nt][1]);
-                mma_elem<kBf16>(acc[nt][c], a[0], a[1], a[2], a[3], pl[i][nt][0], pl[i][nt][1]);
+                float blk[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_elem<kBf16>(blk, a[0], a[1], a[2], a[3], pb[i][nt][0], pb[i][nt][1]);
+                mma_elem<kBf16>(blk, a[0], a[1], a[2], a[3], pl[i][nt][0], pl[i][nt][1]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][c][e] += share[nt][e & 1] * blk[e];
               }
             }
           }

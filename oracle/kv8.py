@@ -76,7 +76,8 @@ def bound(o, spread, reach, dtype, d):
     * a score is a sum of d products with float32 rounding (2^-24 each, some more for its scaling and exponential
       argument): d + 16 roundings of at most `reach`; softmax weights then move by at most twice that, relatively;
     * the exponential itself and the sums: 2^-20;
-    * P in two fp16 parts (2^-22), in two bfloat16 ones (2^-18) beside 16-bit tokens of bfloat16;
+    * P in two fp16 parts (2^-22, or 2^-40 of the largest of the 32 weights that it is taken with: not in the bound, for
+      scores that differ by less than 10), in two bfloat16 ones (2^-18) beside 16-bit tokens of bfloat16;
     * an element below the type's smallest normal number: its absolute step."""
     fi = torch.finfo(dtype)
     p_err = 2.0 ** -18 if dtype == torch.bfloat16 else 2.0 ** -22

@@ -1,6 +1,7 @@
 """Softmax weights of the 8-bit cache's attention (Kv8Cache.attend) where the
 precision that they are held in shows: each weight's own output element, within
-half a step of the output's type.
+half a step of the output's type, and long tails of small weights beside one
+large weight whose value is 0.
 
 Queries have one element other than 0, so that a score is one product and has
 no rounding of a sum of D of them.  Its roundings in float32, each at most
@@ -27,16 +28,17 @@ def _half_step(x, dtype):
     return torch.ldexp(torch.full_like(x, fi.eps / 4), e)  # x = f 2^e, 0.5 <= f < 1
 
 
+@pytest.mark.parametrize("wide", [1, 8])  # scores within 4 and 32 of one another
 @pytest.mark.parametrize("n", [64, 63])  # a block of codes; the 16-bit tokens
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("codes", ["e4m3", "int8"])
-def test_every_weight_is_right_to_half_a_step_of_the_output(dtype, codes, n):
+def test_every_weight_is_right_to_half_a_step_of_the_output(dtype, codes, n, wide):
     """V is the unit matrix: output element j is token j's weight.  A weight held in as many bits as the output adds
     errors of its own and misses the nearest number at every tenth element or so."""
     b, hkv, group, d = 24, 2, 4, 64
     g = torch.Generator(device=DEV).manual_seed(50)
     k, v = torch.zeros(2, b, hkv, n, d, dtype=dtype, device=DEV)
-    k[..., 0] = (2 * torch.rand(b, hkv, n, device=DEV, generator=g) - 1).to(dtype)  # scores within 4 of one another
+    k[..., 0] = (wide * (2 * torch.rand(b, hkv, n, device=DEV, generator=g) - 1)).to(dtype)
     v[...] = torch.eye(d, device=DEV)[:n].to(dtype)
     q = torch.zeros(b, hkv * group, d, dtype=dtype, device=DEV)
     q[..., 0] = (0.5 + 1.5 * torch.rand(b, hkv * group, device=DEV, generator=g)).to(dtype)
@@ -46,8 +48,39 @@ def test_every_weight_is_right_to_half_a_step_of_the_output(dtype, codes, n):
     for i in range(b):
         kk, vv = ok.held(k[i], n, codes), ok.held(v[i], n, codes)
         ref, spread, reach = ok.attend(q[i][:, None], kk, vv, 1, 1.0)
-        # weights in two parts (2^-18 where they are bfloat16), the exponentials and sums 2^-20 each
+        # weights in two parts (2^-18 where they are bfloat16; at least 2^-40 of the largest in fp16 ones), the
+        # exponentials and sums 2^-20 each
         rel = 2 * 6 * 2.0 ** -24 * reach + 2.0 ** -18 + 2 * 2.0 ** -20
-        far = (o[i].double() - ref[:, 0]).abs() - _half_step(ref, dtype)[:, 0] - (rel * spread)[:, 0]
+        far = (o[i].double() - ref[:, 0]).abs() - _half_step(ref, dtype)[:, 0] - (rel * spread)[:, 0] - 2.0 ** -40
         assert far.max().item() <= 0, (i, far.max().item(), (far > 0).double().mean().item())
+    assert pkg.device_error(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("above", [10, 16, 20, 24])  # of the mean, in units of the exponent
+@pytest.mark.parametrize("dtype,codes", [(F16, "e4m3"), (F16, "int8"), (BF16, "e4m3"), (BF16, "int8")])
+@pytest.mark.parametrize("place", [0, 4000, -1])  # in the first block, in the middle, among the 16-bit tokens
+@pytest.mark.parametrize("b,hkv,n,wide", [(64, 32, 8192 + 40, 0.0), (64, 32, 4096 + 7, 2.0), (1, 2, 70_000, 0.0)])
+def test_a_long_tail_beside_one_large_weight(b, hkv, n, wide, place, dtype, codes, above):
+    """An attention sink: one token far above the rest, its value 0, so the output is the tail's.  With 64 x 32 units
+    most workers take a whole one; the long ones are cut into many pieces."""
+    d = 64
+    g = torch.Generator(device=DEV).manual_seed(51)
+    k, v = torch.zeros(2, 1, 1, n, d, dtype=dtype, device=DEV)
+    k[0, 0, :, 0] = (wide * torch.randn(n, device=DEV, generator=g)).to(dtype)
+    k[0, 0, place, 0] = above
+    v[0, 0] = (1 + 0.25 * torch.randn(n, d, device=DEV, generator=g)).to(dtype)
+    v[0, 0, place] = 0
+    cache = pkg.Kv8Cache(b, hkv, n, head_dim=d, dtype=dtype, codes=codes, device=DEV)
+    cache.append(k.expand(b, hkv, n, d), v.expand(b, hkv, n, d))
+    q = torch.zeros(b, hkv, d, dtype=dtype, device=DEV)
+    q[..., 0] = 1
+    o = cache.attend(q, sm_scale=1.0)
+    ref, spread, reach = ok.attend(q[0, :1, None], ok.held(k[0], n, codes), ok.held(v[0], n, codes), 1, 1.0)
+    # Sums: a lane adds every eighth token to the denominator, a sum of the numerator is added to once in 32 tokens
+    # with four roundings of its own; the weights in two parts (2^-18 where they are bfloat16).
+    rel = 2 * 6 * 2.0 ** -24 * reach + (n / 8 + n / 8) * 2.0 ** -24 + 2.0 ** -18 + 2 * 2.0 ** -20
+    # In the 32 tokens that the large weight (at most 1) is among, the others' have an absolute error of 2^-40 of it.
+    near = 32 * 2.0 ** -40 * v.abs().max().item()
+    far = (o[:, :, None].double() - ref).abs() - _half_step(ref, dtype) - rel * spread - near
+    assert far.max().item() <= 0, (far.max().item(), ((o[:, :, None].double() - ref) / ref).abs().max().item())
     assert pkg.device_error(torch.device(DEV)) == 0
