@@ -7,8 +7,8 @@
 // vs * (P . vc).  The codes become fp16 exactly (e4m3 and int8 both fit), so the
 // products run on mma.sync m16n8k16 with fp16 operands and fp32 sums.  Queries
 // enter as fp16 after a power of two per row has brought their largest element
-// into [1, 2): exact for fp16 and for bf16 but for elements 2^-14 below the
-// row's largest, which keep an absolute error of 2^-25 of it.
+// into [2^15, 2^16): exact for fp16, and for bf16 but for elements 2^-32 below
+// the row's largest, which keep an absolute error of 2^-40 of it.
 //
 // Bound by HBM for up to 8 query rows a KV head, which take 16 FLOP a byte (4 x
 // 163,840 tokens, 64 / 8 heads of 128: 214 us, 0.96 of the measured copy rate); by
@@ -222,13 +222,15 @@ __device__ __forceinline__ void lds8(uint32_t addr, uint32_t& lo, uint32_t& hi) 
   // (memory: it may read what plain stores have written)
   asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(lo), "=r"(hi) : "r"(addr) : "memory");
 }
-// A pair of fp16 numbers of 8 significant bits as bf16 (exact).  volatile, so
-// that the conversions of all query fragments stay on the ring's path instead
-// of being kept in registers.
+// A pair of fp16 numbers of 8 significant bits times 2^-15 as bf16 (exact; as
+// they are, the products with bf16 tokens would have no room).  volatile, so that
+// the conversions of all query fragments stay on the ring's path instead of
+// being kept in registers.
 __device__ __forceinline__ uint32_t half_to_bf16(uint32_t x) {
   uint32_t y;
   asm volatile(
       "{\n\t.reg .b16 l, h;\n\t.reg .f32 a, b;\n\tmov.b32 {l, h}, %1;\n\tcvt.f32.f16 a, l;\n\tcvt.f32.f16 b, h;\n\t"
+      "mul.f32 a, a, 0f38000000;\n\tmul.f32 b, b, 0f38000000;\n\t"
       "cvt.rn.bf16x2.f32 %0, b, a;\n\t}"
       : "=r"(y)
       : "r"(x));
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
 
   // ---- the worker's steps.  After a wait that ran out (the error word is
   // set) a warp waits no more, so that it still reaches the CTA's barriers.
-  float qscale[kNT][2];  // of rows 8nt + 2t + (0, 1): the row's power of two, sm_scale and log2(e)
+  float qscale[kNT][2];  // of rows 8nt + 2t + (0, 1): the row's power of two (times 2^14), sm_scale and log2(e)
   float m[kNT][2], l[kNT][2];
   float acc[kNT][kChunks][4];  // dims 16c + g (0, 1) and 16c + g + 8 (2, 3), rows 2t (0, 2) and 2t + 1 (1, 3)
   bool begins = false;         // the piece holds its unit's first step
@@ -611,11 +613,11 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
           }
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          // a power of two from the exponent field; rows of zeros or infinities as they are
+          // a power of two from the exponent field; rows with infinities as they are
           int ex = static_cast<int>(__float_as_uint(top) >> 23);
-          ex = (top == 0.f || ex == 255) ? 127 : min(max(ex, 1), 253);
-          const float f = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
-          const float back = __uint_as_float(static_cast<uint32_t>(ex) << 23) * p.scale_log2;
+          ex = ex == 255 ? 142 : max(ex, 15);
+          const float f = __uint_as_float(static_cast<uint32_t>(269 - ex) << 23);
+          const float back = __uint_as_float(static_cast<uint32_t>(ex - 1) << 23) * p.scale_log2;  // 2^14 / f
 #pragma unroll 2
           for (int c = 0; c < kChunks; ++c) {
             const uint2 x = row[4 * c];
@@ -696,9 +698,11 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
         issue(k + 1, false);
       }
       if (!empty) {
+        const float q_unit = kBf16 && ring ? 2.f : 0x1p-14f;
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt) {
-          const float f0 = s.ks * qscale[nt][0], f1 = s.ks * qscale[nt][1];
+          // (2^-14 last: where it makes the product subnormal, the scores are below 2^-90)
+          const float f0 = s.ks * qscale[nt][0] * q_unit, f1 = s.ks * qscale[nt][1] * q_unit;
 #pragma unroll
           for (int i = 0; i < kTC; ++i)
 #pragma unroll

@@ -84,3 +84,49 @@ def test_a_long_tail_beside_one_large_weight(b, hkv, n, wide, place, dtype, code
     far = (o[:, :, None].double() - ref).abs() - _half_step(ref, dtype) - rel * spread - near
     assert far.max().item() <= 0, (far.max().item(), ((o[:, :, None].double() - ref) / ref).abs().max().item())
     assert pkg.device_error(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("d,dtype,codes", [(64, F16, "e4m3"), (128, F16, "int8"), (64, BF16, "int8"), (128, BF16, "e4m3")])
+@pytest.mark.parametrize("large", [2.0 ** 10, 65504.0, 2.0 ** 18])
+def test_small_query_elements_beside_a_large_one(d, dtype, codes, large):
+    """A query channel far above the others, where the keys are 0: scores are the others' alone, exact to their own
+    roundings (elements 2^-19 to 2^-30 of their row's largest; float16 ends at 65504)."""
+    if dtype == F16 and large > 65504:
+        return
+    b, hkv, group, n = 4, 2, 4, 100
+    small = 2.0 ** -9 if dtype == F16 else 2.0 ** -10
+    g = torch.Generator(device=DEV).manual_seed(52)
+    k, v = torch.randn(2, b, hkv, n, d, device=DEV, generator=g).to(dtype)
+    k[..., 0] = 0
+    q = (small * torch.randn(b, hkv * group, d, device=DEV, generator=g)).to(dtype)
+    q[..., 0] = large
+    scale = 2.0 / (small * d ** 0.5)
+    cache = pkg.Kv8Cache(b, hkv, n, head_dim=d, dtype=dtype, codes=codes, device=DEV)
+    cache.append(k, v)
+    o = cache.attend(q, sm_scale=scale)
+    for i in range(b):
+        ref, spread, reach = ok.attend(q[i][:, None], ok.held(k[i], n, codes), ok.held(v[i], n, codes), 1,
+                                       torch.tensor(scale, dtype=torch.float32).item())
+        far = (o[i].double() - ref[:, 0]).abs() - ok.bound(ref, spread, reach, dtype, d)[:, 0]
+        assert far.max().item() <= 0, (i, far.max().item())
+    assert pkg.device_error(torch.device(DEV)) == 0
+
+
+@pytest.mark.parametrize("dtype,factor", [(F16, 2.0 ** -20), (F16, 2.0 ** 12), (BF16, 2.0 ** -126), (BF16, 2.0 ** -100), (BF16, 2.0 ** 123)])
+def test_queries_at_the_ends_of_their_range(dtype, factor):
+    """Rows whose largest element is among the smallest or largest numbers of the type (also subnormal ones), and zeros."""
+    b, hkv, group, n, d = 2, 2, 4, 100, 64
+    g = torch.Generator(device=DEV).manual_seed(53)
+    k, v = torch.randn(2, b, hkv, n, d, device=DEV, generator=g).to(dtype)
+    q = (factor * torch.randn(b, hkv * group, d, device=DEV, generator=g)).to(dtype)
+    q[:, 1] = 0
+    scale = torch.tensor(0.25 / factor, dtype=torch.float32).item()
+    assert 0 < scale < float("inf")
+    cache = pkg.Kv8Cache(b, hkv, n, head_dim=d, dtype=dtype, device=DEV)
+    cache.append(k, v)
+    o = cache.attend(q, sm_scale=scale)
+    for i in range(b):
+        ref, spread, reach = ok.attend(q[i][:, None], ok.held(k[i], n, "e4m3"), ok.held(v[i], n, "e4m3"), 1, scale)
+        far = (o[i].double() - ref[:, 0]).abs() - ok.bound(ref, spread, reach, dtype, d)[:, 0]
+        assert far.max().item() <= 0, (i, far.max().item())
+    assert pkg.device_error(torch.device(DEV)) == 0
