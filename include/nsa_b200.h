@@ -293,8 +293,8 @@ int nsa_kivi_stream_decode_step_layers(const nsa_kivi_stream_cache* caches, int6
  * scale * code.  A value that is not finite is kept as NaN; its block's scale
  * is then NaN, and attention that sees it is NaN.
  *
- * Pages may be shared by sequences (equal table entries) as long as no call
- * completes a shared block.  A page number outside [0, n_pages), a length or
+ * Pages may be shared by sequences (equal table entries, nsa_kv8_adopt) as
+ * long as no call completes a shared block.  A page number outside [0, n_pages), a length or
  * start outside the table's room, and a start that the ring no longer reaches
  * are recorded in the device error word as NSA_ERR_INVALID: an append then
  * leaves that sequence (for a page number: that block) as it was, attention
@@ -309,7 +309,7 @@ typedef struct {
   int32_t* page_table;
   void *k_ring, *v_ring;
   int64_t* lens;
-  int64_t* ring_floor; /* int64 [batch], zero-filled once: oldest position the ring still holds */
+  int64_t* ring_floor; /* int64 [batch], zero-filled once: how far back the ring reaches, kept by the calls below */
   int32_t* unclean;    /* int32 [batch], zero-filled once: nonzero from a token that is not finite on */
   int32_t* tickets;    /* int32 [batch], zero-filled once; left zero */
 } nsa_kv8_cache;
@@ -323,10 +323,18 @@ typedef struct {
 /* Write counts[b] (NULL: all n_tokens) tokens of new_k / new_v [batch, Hkv,
  * n_tokens, D] at positions starts[b] (NULL: lens[b]) on, quantize the blocks
  * that this completes and set lens[b] = start + count.  A start below lens
- * takes tokens back: any multiple of 64, or a position in the block in which
- * the last append of tokens ended or the one before it. */
+ * takes tokens back: to any multiple of 64, or to a position that the ring
+ * reaches.  It reaches to the block before the one in which the last append
+ * ended, but not below the length that nsa_kv8_adopt set, the last start that
+ * went back further than it reached, or the incomplete block of a length that
+ * was written to lens from outside (its tokens have to be in the ring). */
 int nsa_kv8_append(const nsa_kv8_cache* cache, const nsa_kv8_rows* new_k, const nsa_kv8_rows* new_v, int64_t n_tokens,
                    const int64_t* starts, const int64_t* counts, nsa_stream_t stream);
+/* Let sequence b begin with the lens[b] tokens (int64 [batch]: a multiple of
+ * 64; -1 leaves the sequence as it is) that the pages of its table's first
+ * blocks hold, written by another sequence.  An invalid length is recorded in
+ * the device error word and leaves the sequence as it was. */
+int nsa_kv8_adopt(const nsa_kv8_cache* cache, const int64_t* lens, nsa_stream_t stream);
 /* Read positions starts[b] (NULL: 0) .. + n_tokens of every sequence back into
  * contiguous k_out / v_out [batch, Hkv, n_tokens, D] of out_dtype (0 =
  * float32, 1 = float16, 2 = bfloat16); positions outside [0, lens[b]) are 0. */

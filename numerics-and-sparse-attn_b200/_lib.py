@@ -61,6 +61,7 @@ PROTOTYPES = {
     "nsa_ring_decode": (_INT, [_P, _P, _P, _P] + [_I64] * 6 + [_P, _F, _P, _SZ, _P]),
     "nsa_ring_decode_step": (_INT, [_P, _P, _P, _P] + [_I64] * 6 + [_P, _P, _P, _F, _P, _SZ, _P]),
     "nsa_kv8_append": (_INT, [_P, _P, _P, _I64, _P, _P, _P]),
+    "nsa_kv8_adopt": (_INT, [_P, _P, _P]),
     "nsa_kv8_read": (_INT, [_P, _I64, _P, _P, _P, _INT, _P]),
     "nsa_kv8_workspace_bytes": (_SZ, [_P, _I64, _I64]),
     "nsa_kv8_ticket_count": (_I64, []),

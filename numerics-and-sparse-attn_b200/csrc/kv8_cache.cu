@@ -77,6 +77,15 @@ struct AppendParams {
   int* err;
 };
 
+// ring_floor[b] holds the oldest position of which the ring has the tokens, and
+// the length that an append or adoption left: the ring is known to reach back that
+// far as long as the sequence still has this length.  One that got another by a
+// write to lens (pages of a shared prefix) has its incomplete block there at most.
+__device__ __forceinline__ int64_t ring_state(int64_t floor, int64_t len) { return floor | (len << 32); }
+__device__ __forceinline__ int64_t ring_reach(int64_t state, int64_t len) {
+  return (state >> 32) == len ? (state & 0xffffffff) : len / kBlock * kBlock;
+}
+
 // Where a sequence's new tokens go; ok = 0 leaves it as it was.
 struct Span {
   int start, end, ok;
@@ -142,7 +151,8 @@ __device__ __forceinline__ uint4 ldg16(const uint16_t* p) { return __ldg(reinter
 // `askers` to have read its length sets the new one.
 __device__ __forceinline__ Span take_span(const AppendParams& p, int b, int askers) {
   const Cache& c = p.c;
-  const int64_t len = c.lens[b], cap = int64_t(c.max_blocks) * kBlock, floor = c.ring_floor[b];
+  const int64_t len = c.lens[b], cap = int64_t(c.max_blocks) * kBlock,
+                floor = ring_reach(c.ring_floor[b], len);
   const int64_t s = p.starts ? p.starts[b] : len;
   const int64_t n = p.counts ? p.counts[b] : p.n_tokens;
   const bool ok = s >= 0 && s <= len && len <= cap && n >= 0 && n <= p.n_tokens && s + n <= cap &&
@@ -157,7 +167,7 @@ __device__ __forceinline__ Span take_span(const AppendParams& p, int b, int aske
     if (ok) {
       const int64_t first = s / kBlock * kBlock, last = (s + n) / kBlock * kBlock;
       c.lens[b] = s + n;
-      c.ring_floor[b] = max(s < floor ? first : floor, last - kBlock);
+      c.ring_floor[b] = ring_state(max(s < floor ? first : floor, last - kBlock), s + n);
     }
   }
   return Span{ok ? static_cast<int>(s) : 0, ok ? static_cast<int>(s + n) : 0, ok};
@@ -331,6 +341,23 @@ __global__ void __launch_bounds__(kFewThreads) kv8_append_few_kernel(const Appen
   }
   __syncthreads();  // every thread has read what it needs of the ring
   store_ring<kD, kBf16>(p, b, h, start, end, tid, kFewThreads);
+}
+
+// Sequences begin with pages that hold their first `lens` tokens already; one
+// thread a sequence.
+__global__ void __launch_bounds__(kThreads) kv8_adopt_kernel(const Cache c, const int64_t* lens, int* err) {
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int b = blockIdx.x * kThreads + threadIdx.x;
+  if (b >= c.batch) return;
+  const int64_t n = lens[b];
+  if (n == -1) return;
+  if (n < 0 || n > int64_t(c.max_blocks) * kBlock || n % kBlock) {
+    set_error(err, NSA_ERR_INVALID);
+    return;
+  }
+  c.lens[b] = n;
+  c.ring_floor[b] = ring_state(n, n);  // the ring has nothing of them
 }
 
 // ---------------------------------------------------------------- read back
@@ -509,6 +536,21 @@ extern "C" int nsa_kv8_append(const nsa_kv8_cache* cache, const nsa_kv8_rows* ne
   cudaError_t e = NSA_KV8_DISPATCH(cache, kv8::launch_append, p, stream);
   if (e == cudaSuccess) e = cudaGetLastError();
   return e == cudaSuccess ? NSA_OK : cuda_fail(e, "kv8_append_kernel launch");
+}
+
+extern "C" int nsa_kv8_adopt(const nsa_kv8_cache* cache, const int64_t* lens, nsa_stream_t stream) {
+  clear_error();
+  kv8::Cache c;
+  const int rc = kv8::check_cache(cache, c);
+  if (rc) return rc;
+  if (c.batch == 0) return NSA_OK;
+  if (!lens) return fail(NSA_ERR_INVALID, "lens is NULL");
+  int* const err = device_error_word();
+  if (!err) return fail(NSA_ERR_CUDA, "device error word unavailable");
+  cudaError_t e = launch_kernel(kv8::kv8_adopt_kernel, dim3((c.batch + kv8::kThreads - 1) / kv8::kThreads), dim3(kv8::kThreads),
+                                0, stream, c, lens, err);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  return e == cudaSuccess ? NSA_OK : cuda_fail(e, "kv8_adopt_kernel launch");
 }
 
 extern "C" int nsa_kv8_read(const nsa_kv8_cache* cache, int64_t n_tokens, const int64_t* starts, void* k_out,

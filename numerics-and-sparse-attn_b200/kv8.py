@@ -124,7 +124,8 @@ class Kv8Cache:
     sequence has pages of its own; else a pool of that many pages, which the
     caller hands out by writing page numbers into ``page_table`` (int32
     [batch, blocks], initially 0) before a block is completed.  Sequences may
-    share pages of complete blocks.  ``lens`` (int64 [batch]) holds the lengths.
+    share pages of complete blocks (``adopt``).  ``lens`` (int64 [batch]) holds
+    the lengths.
 
     Storage, readable at any time: ``k_codes`` / ``v_codes`` [n_pages, Hkv, 64,
     D] (float8_e4m3fn or int8), ``scales`` [n_pages, Hkv, 2] float32 (K, V),
@@ -240,8 +241,9 @@ class Kv8Cache:
         with the last dimension contiguous).  ``counts`` (int64 [B]): of the T
         tokens, how many each sequence takes; ``starts`` (int64 [B]): positions
         to write at instead of ``lens``, so that a start below it takes tokens
-        back (any multiple of 64, or as far as the block before the one in
-        which the last append ended)."""
+        back: to any multiple of 64, or as far as the block before the one in
+        which the last append ended, but not into tokens that were adopted or
+        lie below a multiple of 64 that was gone back to further than that."""
         t = self._check("new_k", new_k, self.n_kv_heads)
         if self._check("new_v", new_v, self.n_kv_heads) != t or new_v.dim() != new_k.dim():
             raise ValueError("new_k and new_v must have the same shape")
@@ -253,6 +255,15 @@ class Kv8Cache:
         ``append``'s ``starts`` does (0 empties a sequence)."""
         _req(lens is not None, "lens must be a tensor")
         self._call(self._lib.nsa_kv8_append, None, None, 0, self._words("lens", lens), None)
+
+    def adopt(self, lens):
+        """Let sequence b begin with the ``lens[b]`` tokens (int64 [B], multiples
+        of 64; -1 leaves it as it is) that the pages of its first blocks in
+        ``page_table`` hold, written by another sequence.  Of these, only whole
+        blocks can be taken back (give such a block a page of its own before it
+        is written again)."""
+        _req(lens is not None, "lens must be a tensor")
+        self._call(self._lib.nsa_kv8_adopt, self._words("lens", lens))
 
     # ---------------------------------------------------------------- reading
     def read(self, n_tokens, starts=None, dtype=None):
