@@ -32,12 +32,14 @@ _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 # Scratch of attention.  Eager calls share one (workspace, tickets) pair per
 # (device, stream).  A call captured into a graph takes its workspace from the
-# graph's own pool and one of _GRAPH_ROWS ticket rows (in turn), so that graphs
-# replayed side by side do not share them.
+# graph's own pool and a ticket row for itself, so that graphs replayed side by
+# side do not share them.  A row may be its graph's for as long as the process
+# lives, so it is not handed out again: after _GRAPH_ROWS calls tickets come from
+# the graph's pool, where the graph zeroes them before each (one more node).
 _GRAPH_ROWS = 4096
 _scratch_lock = threading.Lock()
 _eager: dict = {}
-_graph: dict = {}  # device index -> [rows, next]
+_graph: dict = {}  # device index -> [rows, rows handed out]
 
 
 def _graph_rows(device):
@@ -60,10 +62,11 @@ def _capturing(index):
 def _scratch(device, nbytes, stream):
     if _capturing(device.index):
         with _scratch_lock:
-            slot = _graph[device.index]
-            row = slot[1]
-            slot[1] = (row + 1) % _GRAPH_ROWS
-        return torch.empty(nbytes, dtype=torch.uint8, device=device), slot[0][row]
+            rows, row = _graph[device.index]
+            if row < rows.shape[0]:
+                _graph[device.index][1] = row + 1
+        tickets = rows[row] if row < rows.shape[0] else torch.zeros(rows.shape[1], dtype=torch.int32, device=device)
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), tickets
     pair = _eager.get((device.index, stream))
     if pair is None or pair[0].numel() < nbytes:
         with _scratch_lock:
