@@ -80,6 +80,11 @@ def _req(cond, msg, exc=ValueError):
         raise exc(msg)
 
 
+# Tensors that the kernels find by the address that the descriptor holds.
+_STORAGE = frozenset(("k_codes", "v_codes", "scales", "page_table", "k_ring", "v_ring", "lens", "_ring_floor", "_unclean",
+                      "_append_tickets"))
+
+
 class Kv8CacheDesc(ctypes.Structure):
     """ctypes mirror of nsa_kv8_cache (include/nsa_b200.h)."""
     _fields_ = [(n, ctypes.c_int64) for n in ("batch", "n_kv_heads", "head_dim", "n_pages", "max_blocks")] + \
@@ -134,6 +139,9 @@ class Kv8Cache:
     D] (float8_e4m3fn or int8), ``scales`` [n_pages, Hkv, 2] float32 (K, V),
     ``k_ring`` / ``v_ring`` [batch, Hkv, 128, D] (position p at slot p % 128).
 
+    They are written in place (``cache.page_table[b] = pages``); putting another
+    tensor in the place of one is refused.
+
     Calls on one cache are ordered by their stream; calls that write (append,
     decode_step, truncate) must not overlap other calls on the cache.  A page
     number outside the pool, a length or start outside the table's room and a
@@ -179,6 +187,11 @@ class Kv8Cache:
         self._desc_ref = ctypes.byref(d)
         self._lib, self._index, self._ws_bytes = _lib.load(), device.index, {}
         _graph_rows(device)
+
+    def __setattr__(self, name, value):
+        if name in _STORAGE and self.__dict__.get(name, value) is not value:
+            raise AttributeError(f"{name} is the cache's storage: write into it (indexing, copy_), it cannot be replaced")
+        super().__setattr__(name, value)
 
     # ---------------------------------------------------------------- plumbing
     # (messages are built where they are raised: these checks run on every call)
