@@ -236,7 +236,8 @@ class Kv8Cache:
         """Workspace and tickets of one attend."""
         nbytes = self._ws_bytes.get((heads, n_tokens))
         if nbytes is None:
-            nbytes = self._lib.nsa_kv8_workspace_bytes(self._desc_ref, heads, n_tokens)
+            with _lib.on_device(self.device):  # (it depends on the device's number of SMs)
+                nbytes = self._lib.nsa_kv8_workspace_bytes(self._desc_ref, heads, n_tokens)
             if self.batch and not nbytes:
                 _lib.check(_lib.NSA_ERR_INVALID)  # raises with the library's message
             self._ws_bytes[heads, n_tokens] = nbytes
