@@ -310,7 +310,7 @@ typedef struct {
   void *k_ring, *v_ring;
   int64_t* lens;
   int64_t* ring_floor; /* int64 [batch], zero-filled once: how far back the ring reaches, kept by the calls below */
-  int32_t* unclean;    /* int32 [batch], zero-filled once: nonzero from a token that is not finite on */
+  int32_t* unclean;    /* int32 [batch], zero-filled once: which heads' rings may hold values that are not finite */
   int32_t* tickets;    /* int32 [batch], zero-filled once; left zero */
 } nsa_kv8_cache;
 /* Rows of head_dim elements; strides in elements (multiples of 8, data

@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(Shape<kD, kNT>::kThreads, 1)
     } else {
       ahead.pos0 = s.full * kBlock + (step - blocks) * kRingTok;
       ahead.row = (b * p.c.n_kv_heads + h) * kRing + ahead.pos0 % kRing;
-      flags |= kRingStep | kMasked | (p.c.unclean[b] ? kUnclean : 0) | (min(kRingTok, s.len - ahead.pos0) << 16);
+      flags |= kRingStep | kMasked | (p.c.unclean[b] >> (h & 31) & 1 ? kUnclean : 0) | (min(kRingTok, s.len - ahead.pos0) << 16);
     }
     ahead.flags = flags;
   };

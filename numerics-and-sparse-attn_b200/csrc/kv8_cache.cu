@@ -89,6 +89,7 @@ __device__ __forceinline__ int64_t ring_reach(int64_t state, int64_t len) {
 // Where a sequence's new tokens go; ok = 0 leaves it as it was.
 struct Span {
   int start, end, ok;
+  int anew;  // the ring holds nothing of the tokens before
 };
 
 // max(m, |x|) over the 8 elements of x; NaN stays.
@@ -158,11 +159,14 @@ __device__ __forceinline__ Span take_span(const AppendParams& p, int b, int aske
   const bool ok = s >= 0 && s <= len && len <= cap && n >= 0 && n <= p.n_tokens && s + n <= cap &&
                   (s % kBlock == 0 || s >= floor);
   if (!ok) set_error(p.err, NSA_ERR_INVALID);
-  // The ticket's step is made from `ok` (the same for all of a sequence's askers):
-  // it cannot be taken before what this thread needs of lens and floor is there.
-  // (A fence in its place costs 0.8 us a call, 13 us in a prompt of 8000 tokens.)
-  const int step = ok ? 1 : 2;
-  if (atomicAdd(c.tickets + b, step) == (askers - 1) * step) {
+  const bool anew = ok && s <= floor;
+  // The ticket's step is made from `ok` and `anew` (the same for all of a sequence's
+  // askers): it cannot be taken before what this thread needs of lens and floor is there.
+  // That is an order of the machine, which does not guess the operand of an atomic;
+  // the memory model would ask for a release, which costs 7 us in a prompt of 8000
+  // tokens (129 us) and 0.8 in a step of 256 sequences.
+  const unsigned step = anew ? 1 : ok ? 2 : 3;
+  if (atomicAdd(reinterpret_cast<unsigned*>(c.tickets + b), step) == (askers - 1) * step) {
     c.tickets[b] = 0;
     if (ok) {
       const int64_t first = s / kBlock * kBlock, last = (s + n) / kBlock * kBlock;
@@ -170,7 +174,7 @@ __device__ __forceinline__ Span take_span(const AppendParams& p, int b, int aske
       c.ring_floor[b] = ring_state(max(s < floor ? first : floor, last - kBlock), s + n);
     }
   }
-  return Span{ok ? static_cast<int>(s) : 0, ok ? static_cast<int>(s + n) : 0, ok};
+  return Span{ok ? static_cast<int>(s) : 0, ok ? static_cast<int>(s + n) : 0, ok, anew};
 }
 
 // Quantizes block i of a unit, which a whole CTA calls for: its tokens from
@@ -232,6 +236,14 @@ __device__ __forceinline__ void quantize_block(const AppendParams& p, int b, int
   if (tid == 0) c.scales[rec] = make_float2(kbad ? NAN : ks, vbad ? NAN : vs);
 }
 
+// A KV head's bit in unclean[b] says that its ring may hold a value that is not
+// finite.  It is taken back where the ring begins anew, by the unit's CTA before
+// that stores to it (with more than 32 heads two CTAs have a bit: it stays).
+__device__ __forceinline__ int unclean_bit(int h) { return 1 << (h & 31); }
+__device__ __forceinline__ void ring_anew(const Cache& c, const Span& span, int b, int h) {
+  if (span.anew && c.n_kv_heads <= 32) atomicAnd(c.unclean + b, ~unclean_bit(h));
+}
+
 // Stores a unit's tokens of its last two blocks in the ring, as they came;
 // threads `id` of `n` share the rows.
 template <int kD, bool kBf16>
@@ -252,7 +264,7 @@ __device__ __forceinline__ void store_ring(const AppendParams& p, int b, int h, 
       *w[e] |= mk & 0x7fff7fffu;  // NaN
       bad |= mk;
     }
-    if (bad) c.unclean[b] = 1;
+    if (bad) atomicOr(c.unclean + b, unclean_bit(h));
     *reinterpret_cast<uint4*>(c.k_ring + ring + (pos % kRing) * kD) = k;
     *reinterpret_cast<uint4*>(c.v_ring + ring + (pos % kRing) * kD) = v;
   }
@@ -269,7 +281,10 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(const AppendParams
   grid_launch_dependents();
   grid_dependency_wait();
   const int tid = threadIdx.x, b = blockIdx.x / p.c.n_kv_heads, h = blockIdx.x % p.c.n_kv_heads;
-  if (tid == 0) span = take_span(p, b, p.c.n_kv_heads * gridDim.y);
+  if (tid == 0) {
+    span = take_span(p, b, p.c.n_kv_heads * gridDim.y);
+    if (blockIdx.y == 0) ring_anew(p.c, span, b, h);
+  }
   __syncthreads();
   if (!span.ok) return;
   const int start = span.start, end = span.end;
@@ -298,7 +313,10 @@ __global__ void __launch_bounds__(kFewThreads) kv8_append_few_kernel(const Appen
   grid_dependency_wait();
   const Cache& c = p.c;
   const int tid = threadIdx.x, b = blockIdx.x / c.n_kv_heads, h = blockIdx.x % c.n_kv_heads;
-  if (tid == 0) span = take_span(p, b, c.n_kv_heads);
+  if (tid == 0) {
+    span = take_span(p, b, c.n_kv_heads);
+    ring_anew(c, span, b, h);
+  }
   __syncthreads();
   if (!span.ok) return;
   const int start = span.start, end = span.end, i = start / kBlock;
@@ -358,6 +376,7 @@ __global__ void __launch_bounds__(kThreads) kv8_adopt_kernel(const Cache c, cons
   }
   c.lens[b] = n;
   c.ring_floor[b] = ring_state(n, n);  // the ring has nothing of them
+  c.unclean[b] = 0;
 }
 
 // ---------------------------------------------------------------- read back
@@ -486,7 +505,7 @@ cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
                          0, stream, p);
   }
   const int more = (p.n_tokens + kBlock - 1) / kBlock;  // blocks besides a unit's first
-  int most = (1 << 30) / p.c.n_kv_heads - 2;  // twice a sequence's CTAs is an int
+  int most = (1 << 30) / p.c.n_kv_heads - 2;  // three times a sequence's CTAs is an unsigned
   most = most < 65534 ? most : 65534;
   const dim3 grid(static_cast<unsigned>(units), 1 + static_cast<unsigned>(more < most ? more : most));
   return launch_kernel(kv8_append_kernel<kD, kBf16, kInt8>, grid, dim3(kThreads), 0, stream, p);
