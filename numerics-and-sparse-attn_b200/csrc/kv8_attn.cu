@@ -11,8 +11,8 @@
 // the row's largest, which keep an absolute error of 2^-40 of it.
 //
 // Bound by HBM for up to 8 query rows a KV head, which take 16 FLOP a byte (4 x
-// 163,840 tokens, 64 / 8 heads of 128: 214 us, 0.96 of the measured copy rate); by
-// the instructions around the products for more (32 rows: 0.31).  tcgen05 would
+// 163,840 tokens, 64 / 8 heads of 128: 211 us, 0.98 of the measured copy rate); by
+// the instructions around the products for more (32 rows: 0.26).  tcgen05 would
 // want the codes as fp16 in shared memory first and tiles of 64 or 128 rows; here
 // the conversion happens in registers on the way from ldmatrix to the mma.
 // Short calls are bound by the way from the lengths to the first load (3 us from
@@ -1044,7 +1044,7 @@ int max_ctas() {
   return sms > 0 ? sms : 148;
 }
 
-// Query rows of a unit: up to 8, 16 or 32; more of them are further units.
+// Query rows of a unit: 8 or 16; more of them are further units.
 Plan plan(const nsa_kv8_cache* c, int64_t rows) {
   Plan s;
   s.nt = rows <= 8 ? 1 : 2;

@@ -422,7 +422,7 @@ __device__ __forceinline__ void store8(void* out, int64_t at, const float (&x)[8
 // One CTA a tile of kReadRows positions of a unit; a thread takes 8 elements of a
 // row of K and of V, so that a warp's 16-byte stores fill whole sectors.  Bound
 // by HBM (1 byte in, 2 out an element): all of a thread's loads are issued before
-// its stores.  8 x 16,000 tokens, 8 heads of 128 to bf16: 123 us, 0.98 of the
+// its stores.  8 x 16,000 tokens, 8 heads of 128 to bf16: 124 us, 0.97 of the
 // measured copy rate (16 elements a thread, each store half a sector a lane: 146;
 // CTAs that take tiles in turn and look the next one's pages up ahead: 166).
 constexpr int kReadRows = 64;

@@ -143,7 +143,7 @@ class Kv8Cache:
     tensor in the place of one is refused.
 
     Calls on one cache are ordered by their stream; calls that write (append,
-    decode_step, truncate) must not overlap other calls on the cache.  A page
+    decode_step, truncate, adopt) must not overlap other calls on the cache.  A page
     number outside the pool, a length or start outside the table's room and a
     start that the ring no longer reaches are reported by ``device_error()``.
     """
