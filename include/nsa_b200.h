@@ -284,7 +284,7 @@ int nsa_kivi_stream_decode_step_layers(const nsa_kivi_stream_cache* caches, int6
  *   ring    f16/bf16 [batch, Hkv, 128, D], K and V apart: position p at slot
  *           p % 128 holds the tokens of the incomplete block as they came, and
  *           keeps those of the block before it
- *   lens    int64 [batch]: tokens of each sequence
+ *   lens    int64 [batch]: tokens of each sequence, set by the calls below
  *
  * Complete blocks are read as codes, the up to 63 tokens behind them from the
  * ring, so what the cache holds depends on the tokens alone, not on how calls

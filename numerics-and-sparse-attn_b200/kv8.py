@@ -133,14 +133,15 @@ class Kv8Cache:
     caller hands out by writing page numbers into ``page_table`` (int32
     [batch, blocks], initially 0) before a block is completed.  Sequences may
     share pages of complete blocks (``adopt``).  ``lens`` (int64 [batch]) holds
-    the lengths.
+    the lengths, which the calls set; who writes one has to see to the ring's
+    tokens of an incomplete block as well.
 
     Storage, readable at any time: ``k_codes`` / ``v_codes`` [n_pages, Hkv, 64,
     D] (float8_e4m3fn or int8), ``scales`` [n_pages, Hkv, 2] float32 (K, V),
     ``k_ring`` / ``v_ring`` [batch, Hkv, 128, D] (position p at slot p % 128).
 
-    They are written in place (``cache.page_table[b] = pages``); putting another
-    tensor in the place of one is refused.
+    The table and the storage are written in place (``cache.page_table[b] =
+    pages``); putting another tensor in the place of one is refused.
 
     Calls on one cache are ordered by their stream; calls that write (append,
     decode_step, truncate, adopt) must not overlap other calls on the cache.  A page
